@@ -1,0 +1,178 @@
+// Launches and C ABI of linear attention (linattn.hpp).
+#include <climits>
+
+#include "linattn.hpp"
+#include "ops_status.hpp"
+
+namespace sffft {
+namespace {
+
+using la::March;
+using la::Operand;
+using la::Shape;
+
+constexpr int MAX_D = 128;
+
+bool valid_shape(const sffft_linattn* p) {
+  if (!p || !ops::valid_io(p->io) || p->B < 1 || p->T < 1 || p->H < 1 || p->Hk < 1 || p->H % p->Hk) return false;
+  if (p->Dk < 8 || p->Dv < 8 || p->Dk > MAX_D || p->Dv > MAX_D || p->Dk % 8 || p->Dv % 8) return false;
+  return (long long)p->B * p->H <= INT_MAX / 64 && (long long)p->B * p->T <= INT_MAX;
+}
+
+// A strided input: 16-byte aligned rows, and its extent.
+bool valid_input(const void* x, const long long s[3], const sffft_linattn* p, int heads, int D, size_t* bytes) {
+  const int elem = p->io ? 2 : 4;
+  if (!x || !ops::aligned(x, 16)) return false;
+  for (int i = 0; i < 3; i++)
+    if (s[i] * elem % 16) return false;
+  *bytes = ops::extent(s, p->B, p->T, heads, D, elem);
+  return *bytes != 0;
+}
+
+Operand operand(const void* x, const long long s[3], int div) { return {x, s[0], s[1], s[2], div}; }
+
+template <class T>
+hipError_t recur(const March& m, const Shape& s, hipStream_t st) {
+  hipLaunchKernelGGL(la::recur_kernel<T>, dim3((unsigned)(s.B * s.H * ((m.V + 15) / 16))), dim3(64), 0, st, m, s);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t head_sum(const float* in, void* out, long long n, int D, int G, hipStream_t st) {
+  hipLaunchKernelGGL(la::head_sum_kernel<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, in,
+                     static_cast<T*>(out), n, D, G);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const void* v, const Shape& s,
+                   const float* s0, void* o, float* s1, hipStream_t st) {
+  const int G = p->H / p->Hk;
+  return recur<T>({operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, s1, p->Dk, p->Dv, p->Dv, 1, 0,
+                   0, p->scale, p->scale, 1.f},
+                  s, st);
+}
+
+// dk and dv of heads that are shared, for each query head, before their sum
+size_t shared_bytes(const sffft_linattn* p) {
+  return p->H == p->Hk ? 0 : (size_t)p->B * p->T * p->H * (p->Dk + p->Dv) * 4;
+}
+
+template <class T>
+hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const void* v, const void* go,
+                    const Shape& s, const float* s0, const float* ds1, void* dq, void* dk, void* dv, float* ds0,
+                    float* work, hipStream_t st) {
+  const int G = p->H / p->Hk;
+  const Operand Q = operand(q, p->q, 1), K = operand(k, p->k, G), V = operand(v, p->v, G), O = operand(go, p->go, 1);
+  const size_t rows = (size_t)p->B * p->T;
+  float *wk = work, *wv = work + rows * p->H * p->Dk;
+  const float c = p->scale;
+  hipError_t e = recur<T>({O, V, K, dq, s0, nullptr, p->Dv, p->Dk, 1, p->Dv, 0, 0, c, c, 1.f}, s, st);
+  if (e == hipSuccess)
+    e = recur<T>({K, Q, O, G > 1 ? wv : dv, ds1, ds0, p->Dk, p->Dv, p->Dv, 1, 1, G > 1, c, 1.f, c}, s, st);
+  if (e == hipSuccess)
+    e = recur<T>({V, O, Q, G > 1 ? wk : dk, ds1, nullptr, p->Dv, p->Dk, 1, p->Dv, 1, G > 1, c, 1.f, c}, s, st);
+  if (e == hipSuccess && G > 1) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * p->Dk, p->Dk, G, st);
+  if (e == hipSuccess && G > 1) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * p->Dv, p->Dv, G, st);
+  return e;
+}
+
+}  // namespace
+}  // namespace sffft
+
+using namespace sffft;
+
+extern "C" {
+
+size_t sffft_linattn_work_bytes(const sffft_linattn* p, int backward) {
+  if (!valid_shape(p)) return 0;
+  return backward ? shared_bytes(p) : 0;
+}
+
+int sffft_linattn_fwd(const sffft_linattn* p, const void* q, const void* k, const void* v, const float* log_decay,
+                      const float* initial_state, const int* lengths, void* o, float* final_state, void* work,
+                      size_t work_bytes, void* stream) {
+  size_t nq, nk, nv;
+  if (!valid_shape(p) || !log_decay || !o || !ops::aligned(o, 16) || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
+      !valid_input(k, p->k, p, p->Hk, p->Dk, &nk) || !valid_input(v, p->v, p, p->Hk, p->Dv, &nv) ||
+      !ops::aligned(initial_state, 16) || !ops::aligned(final_state, 16) || !ops::aligned(log_decay, 4) ||
+      !ops::aligned(lengths, 4))
+    return SFFFT_EINVAL;
+  const size_t no = (size_t)p->B * p->T * p->H * p->Dv * (p->io ? 2 : 4), ns = (size_t)p->B * p->H * p->Dk * p->Dv * 4;
+  const void* in[] = {q, k, v, initial_state};
+  const size_t len[] = {nq, nk, nv, ns};
+  for (int i = 0; i < 4; i++)
+    if (ops::overlap(o, no, in[i], len[i]) || ((i < 3 || in[i] != final_state) && ops::overlap(final_state, ns, in[i], len[i])))
+      return SFFFT_EINVAL;
+  if (ops::overlap(o, no, final_state, ns)) return SFFFT_EINVAL;
+  const size_t need = sffft_linattn_work_bytes(p, 0);
+  if (need && (!work || work_bytes < need || !ops::aligned(work, 16) || ops::overlap(work, need, o, no) ||
+               ops::overlap(work, need, final_state, ns)))
+    return SFFFT_EINVAL;
+  for (int i = 0; i < 4; i++)
+    if (need && ops::overlap(work, need, in[i], len[i])) return SFFFT_EINVAL;
+  const Shape s = {p->B, p->T, p->H, log_decay, lengths};
+  const auto run = p->io ? forward<uint16_t> : forward<float>;
+  return ops::hip_status(run(p, q, k, v, s, initial_state, o, final_state, (hipStream_t)stream),
+                         "linear attention launch");
+}
+
+int sffft_linattn_bwd(const sffft_linattn* p, const void* q, const void* k, const void* v, const float* log_decay,
+                      const float* initial_state, const int* lengths, const void* go, const float* d_final_state,
+                      void* dq, void* dk, void* dv, float* d_initial_state, void* work, size_t work_bytes,
+                      void* stream) {
+  size_t nq, nk, nv, no;
+  if (!valid_shape(p) || !log_decay || !dq || !dk || !dv || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
+      !valid_input(k, p->k, p, p->Hk, p->Dk, &nk) || !valid_input(v, p->v, p, p->Hk, p->Dv, &nv) ||
+      !valid_input(go, p->go, p, p->H, p->Dv, &no) || !ops::aligned(initial_state, 16) ||
+      !ops::aligned(d_final_state, 16) || !ops::aligned(d_initial_state, 16) || !ops::aligned(dq, 16) ||
+      !ops::aligned(dk, 16) || !ops::aligned(dv, 16) || !ops::aligned(log_decay, 4) || !ops::aligned(lengths, 4))
+    return SFFFT_EINVAL;
+  const size_t elem = p->io ? 2 : 4, rows = (size_t)p->B * p->T, ns = (size_t)p->B * p->H * p->Dk * p->Dv * 4;
+  const size_t need = sffft_linattn_work_bytes(p, 1);
+  if (need && (!work || work_bytes < need || !ops::aligned(work, 16))) return SFFFT_EINVAL;
+  const void* in[] = {q, k, v, go, initial_state, d_final_state};
+  const size_t len[] = {nq, nk, nv, no, ns, ns};
+  const void* out[] = {dq, dk, dv, d_initial_state, need ? work : nullptr};
+  const size_t size[] = {rows * p->H * p->Dk * elem, rows * p->Hk * p->Dk * elem, rows * p->Hk * p->Dv * elem, ns, need};
+  for (int i = 0; i < 5; i++) {
+    for (int j = 0; j < 6; j++)
+      if (ops::overlap(out[i], size[i], in[j], len[j])) return SFFFT_EINVAL;
+    for (int j = 0; j < i; j++)
+      if (ops::overlap(out[i], size[i], out[j], size[j])) return SFFFT_EINVAL;
+  }
+  const Shape s = {p->B, p->T, p->H, log_decay, lengths};
+  const auto run = p->io ? backward<uint16_t> : backward<float>;
+  return ops::hip_status(run(p, q, k, v, go, s, initial_state, d_final_state, dq, dk, dv, d_initial_state,
+                             static_cast<float*>(work), (hipStream_t)stream),
+                         "linear attention gradient launch");
+}
+
+int sffft_linattn_step(const sffft_linattn* p, const void* q, const void* k, const void* v, const float* log_decay,
+                       float* state, int slots, const int* slot, void* o, void* stream) {
+  size_t nq, nk, nv;
+  if (!valid_shape(p) || p->T != 1 || !log_decay || !state || !o || slots < 1 || !ops::aligned(state, 16) ||
+      !ops::aligned(o, 16) || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
+      !valid_input(k, p->k, p, p->Hk, p->Dk, &nk) || !valid_input(v, p->v, p, p->Hk, p->Dv, &nv) ||
+      !ops::aligned(log_decay, 4) || !ops::aligned(slot, 4))
+    return SFFFT_EINVAL;
+  const size_t no = (size_t)p->B * p->H * p->Dv * (p->io ? 2 : 4), ns = (size_t)slots * p->H * p->Dk * p->Dv * 4;
+  const void* in[] = {q, k, v};
+  const size_t len[] = {nq, nk, nv};
+  for (int i = 0; i < 3; i++)
+    if (ops::overlap(o, no, in[i], len[i]) || ops::overlap(state, ns, in[i], len[i])) return SFFFT_EINVAL;
+  if (ops::overlap(o, no, state, ns)) return SFFFT_EINVAL;
+  const int G = p->H / p->Hk;
+  const Operand Q = operand(q, p->q, 1), K = operand(k, p->k, G), V = operand(v, p->v, G);
+  const dim3 grid((unsigned)(p->B * p->H), (unsigned)((p->Dv + 63) / 64)), block(256);
+  hipStream_t st = (hipStream_t)stream;
+  if (p->io)
+    hipLaunchKernelGGL(la::step_kernel<uint16_t>, grid, block, 0, st, Q, K, V, log_decay, state, slots, slot,
+                       static_cast<uint16_t*>(o), p->H, p->Dk, p->Dv, p->scale);
+  else
+    hipLaunchKernelGGL(la::step_kernel<float>, grid, block, 0, st, Q, K, V, log_decay, state, slots, slot,
+                       static_cast<float*>(o), p->H, p->Dk, p->Dv, p->scale);
+  return ops::hip_status(hipGetLastError(), "linear attention step launch");
+}
+
+}  // extern "C"

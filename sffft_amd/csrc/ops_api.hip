@@ -1,0 +1,329 @@
+// Launches and C ABI of the rotary positions (rotary.hpp) and of the norms around a block
+// (blocknorm.hpp), and the error text of the library.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdio>
+
+#include "blocknorm.hpp"
+#include "ops_status.hpp"
+#include "rotary.hpp"
+
+namespace sffft {
+namespace ops {
+
+thread_local char g_last_error[256] = "";
+
+int hip_status(hipError_t err, const char* what) {
+  if (err == hipSuccess) return SFFFT_OK;
+  snprintf(g_last_error, sizeof(g_last_error), "%s: %s (%d)", what, hipGetErrorString(err), (int)err);
+  return SFFFT_EHIP;
+}
+
+}  // namespace ops
+
+namespace {
+
+// ---- rotary ----
+
+template <class T>
+hipError_t rotary(rot::Args a, long long tokens, bool interleaved, bool wide, hipStream_t st) {
+  constexpr int PP = 16 / sizeof(T);
+  const int pp = wide ? PP : 1;
+  a.items = tokens * a.heads * (a.D / (2 * pp));
+  const dim3 grid((unsigned)((a.items + 255) / 256)), block(256);
+  if (wide) {
+    if (interleaved) hipLaunchKernelGGL((rot::rotary_kernel<T, PP, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rot::rotary_kernel<T, PP, false>), grid, block, 0, st, a);
+  } else {
+    if (interleaved) hipLaunchKernelGGL((rot::rotary_kernel<T, 1, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rot::rotary_kernel<T, 1, false>), grid, block, 0, st, a);
+  }
+  return hipGetLastError();
+}
+
+// ---- norms ----
+
+// How a row lies in registers: VEC channels to a load, NV loads to a lane, `lanes` lanes to a row; the
+// fewest lanes that hold it in 16 channels each. Four rows to a workgroup where one wavefront holds a row.
+struct RowShape {
+  int vec, nv, lanes, block;
+};
+RowShape row_shape(int C, bool wide) {
+  RowShape s;
+  s.vec = wide ? 4 : 1;
+  s.lanes = 64;
+  while (s.lanes * 16 < C) s.lanes *= 2;
+  const int per = (C + s.lanes - 1) / s.lanes;  // channels of a lane
+  s.nv = (per + 3) / 4;                         // in fours, whatever the loads
+  s.block = s.lanes == 64 ? 256 : s.lanes;
+  return s;
+}
+
+// Rows in parts that one workgroup each takes: about 8 wavefronts for each of 256 CUs, no part across
+// rows of different gates.
+struct Parts {
+  long long block_rows, blocks, nparts;
+  int part_rows, per_block;
+};
+Parts parts_of(const sffft_blocknorm* p, const RowShape& s, bool shared_gate) {
+  Parts q;
+  q.block_rows = shared_gate ? p->gate_rows : p->rows;
+  q.blocks = p->rows / q.block_rows;
+  const int at_once = s.lanes == 64 ? 4 : 1;
+  const long long want = std::max<long long>(1, 256 * 8 * 64 / s.block / q.blocks);
+  const long long rounds = (q.block_rows + at_once - 1) / at_once;
+  long long per = std::min(want, rounds);
+  q.part_rows = (int)std::min<long long>((rounds + per - 1) / per * at_once, INT_MAX / 2);
+  q.per_block = (int)((q.block_rows + q.part_rows - 1) / q.part_rows);
+  q.nparts = q.blocks * q.per_block;
+  return q;
+}
+
+template <class T, int VEC, int NV, int BLK>
+void norm_launch(const bn::Args& a, bool y, bool backward, dim3 grid, dim3 block, hipStream_t st) {
+  if (backward) {
+    if (y) hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, NV, BLK, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, NV, BLK, false>), grid, block, 0, st, a);
+  } else {
+    if (y) hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, NV, BLK, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, NV, BLK, false>), grid, block, 0, st, a);
+  }
+}
+template <class T, int VEC, int BLK>
+void norm_nv(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
+  constexpr int Q = 4 / VEC;
+  const dim3 block((unsigned)s.block);
+  switch (s.nv) {
+    case 1: return norm_launch<T, VEC, Q, BLK>(a, y, backward, grid, block, st);
+    case 2: return norm_launch<T, VEC, 2 * Q, BLK>(a, y, backward, grid, block, st);
+    case 3: return norm_launch<T, VEC, 3 * Q, BLK>(a, y, backward, grid, block, st);
+    default: return norm_launch<T, VEC, 4 * Q, BLK>(a, y, backward, grid, block, st);
+  }
+}
+template <class T>
+hipError_t norm(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
+  if (s.vec == 4) {
+    if (s.block <= 256) norm_nv<T, 4, 256>(a, s, y, backward, grid, st);
+    else norm_nv<T, 4, 1024>(a, s, y, backward, grid, st);
+  } else {
+    if (s.block <= 256) norm_nv<T, 1, 256>(a, s, y, backward, grid, st);
+    else norm_nv<T, 1, 1024>(a, s, y, backward, grid, st);
+  }
+  return hipGetLastError();
+}
+
+constexpr int MAX_C = 16384;
+
+bool valid_norm(const sffft_blocknorm* p) {
+  return p && ops::valid_io(p->io) && p->rows >= 1 && p->rows <= (1LL << 40) && p->C >= 1 && p->C <= MAX_C &&
+         p->act >= SFFFT_ACT_NONE && p->act <= SFFFT_ACT_SILU && p->gate_rows >= 1 && p->rows % p->gate_rows == 0 &&
+         p->eps >= 0.f && std::isfinite(p->eps);
+}
+
+// extents of the rows of a strided array; 0 if invalid
+size_t row_bytes(const sffft_blocknorm* p, long long stride, long long rows) {
+  if (stride < 0 || (rows > 1 && stride && stride < p->C)) return 0;
+  const __int128 e = ((__int128)stride * (rows - 1) + p->C) * (p->io ? 2 : 4);
+  return e >= ((__int128)1 << 62) ? 0 : (size_t)e;
+}
+
+struct Span {
+  const void* p;
+  size_t n;
+};
+// no output overlaps an input or another output
+bool apart(const Span* in, int ni, const Span* out, int no) {
+  for (int i = 0; i < no; i++) {
+    for (int j = 0; j < ni; j++)
+      if (ops::overlap(out[i].p, out[i].n, in[j].p, in[j].n)) return false;
+    for (int j = 0; j < i; j++)
+      if (ops::overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return false;
+  }
+  return true;
+}
+
+// Vector loads of four channels: every array's rows aligned to them.
+bool wide_rows(const sffft_blocknorm* p, const Span* all, int n, const long long* strides, int ns) {
+  const int elem = p->io ? 2 : 4;
+  if (p->C % 4) return false;
+  for (int i = 0; i < n; i++)
+    if (!ops::aligned(all[i].p, 4 * elem)) return false;
+  for (int i = 0; i < ns; i++)
+    if (strides[i] % 4) return false;
+  return true;
+}
+
+}  // namespace
+}  // namespace sffft
+
+using namespace sffft;
+
+extern "C" {
+
+int sffft_rotary_apply(const sffft_rotary* p, const void* q, const void* k, const float* table, const void* pos,
+                       void* qo, void* ko, void* stream) {
+  if (!p || !ops::valid_io(p->io) || p->B < 1 || p->T < 1 || p->H < 1 || p->Hk < 0 || p->D < 2 || p->D % 2 ||
+      p->R < 2 || p->R % 2 || p->R > p->D || p->positions < 1 || (p->interleaved != 0 && p->interleaved != 1) ||
+      (p->inverse != 0 && p->inverse != 1) || (pos && p->pos_bits != 32 && p->pos_bits != 64) || !q || !qo || !table ||
+      (p->Hk > 0) != (k != nullptr) || (p->Hk > 0) != (ko != nullptr))
+    return SFFFT_EINVAL;
+  const int elem = p->io ? 2 : 4;
+  const __int128 items = (__int128)p->B * p->T * ((__int128)p->H + p->Hk) * (p->D / 2);
+  if (items > (__int128)INT_MAX * 128 || (long long)p->H + p->Hk > INT_MAX) return SFFFT_EINVAL;
+  const size_t nq = ops::extent(p->q, p->B, p->T, p->H, p->D, elem), mq = ops::extent(p->qo, p->B, p->T, p->H, p->D, elem);
+  const size_t nk = k ? ops::extent(p->k, p->B, p->T, p->Hk, p->D, elem) : 1;
+  const size_t mk = k ? ops::extent(p->ko, p->B, p->T, p->Hk, p->D, elem) : 1;
+  if (!nq || !mq || !nk || !mk || !ops::aligned(q, elem) || !ops::aligned(k, elem) || !ops::aligned(qo, elem) ||
+      !ops::aligned(ko, elem) || !ops::aligned(table, 4) || !ops::aligned(pos, p->pos_bits / 8))
+    return SFFFT_EINVAL;
+  // in place (q itself, with its strides) or apart
+  const bool sq = q == qo && std::equal(p->q, p->q + 3, p->qo), sk = k == ko && std::equal(p->k, p->k + 3, p->ko);
+  const size_t nt = (size_t)p->positions * p->R * 4, np = pos ? (size_t)p->B * p->T * (p->pos_bits / 8) : 0;
+  // (in place, q and k may be views of one array whose extents interleave)
+  if ((!sq && (ops::overlap(qo, mq, q, nq) || ops::overlap(qo, mq, k, k ? nk : 0))) ||
+      (!sk && (ops::overlap(ko, mk, k, nk) || ops::overlap(ko, k ? mk : 0, q, nq))) || qo == ko ||
+      ops::overlap(qo, mq, table, nt) ||
+      ops::overlap(ko, mk, table, nt) || ops::overlap(qo, mq, pos, np) || ops::overlap(ko, mk, pos, np))
+    return SFFFT_EINVAL;
+  rot::Args a = {};
+  a.q = {q, qo, p->q[0], p->q[1], p->q[2], p->qo[0], p->qo[1], p->qo[2]};
+  a.k = {k, ko, p->k[0], p->k[1], p->k[2], p->ko[0], p->ko[1], p->ko[2]};
+  a.table = table, a.pos = pos, a.pos64 = p->pos_bits == 64, a.positions = p->positions;
+  a.T = p->T, a.H = p->H, a.heads = p->H + p->Hk, a.D = p->D, a.R = p->R, a.inverse = p->inverse;
+  // 16-byte loads of 8 bf16 or 4 fp32 channels; a lane takes two
+  bool wide = p->D % (32 / elem) == 0 && p->R % (32 / elem) == 0 && ops::aligned(q, 16) && ops::aligned(k, 16) &&
+              ops::aligned(qo, 16) && ops::aligned(ko, 16) && ops::aligned(table, 16);
+  for (int i = 0; i < 3; i++)
+    wide = wide && p->q[i] * elem % 16 == 0 && p->qo[i] * elem % 16 == 0 &&
+           (!k || (p->k[i] * elem % 16 == 0 && p->ko[i] * elem % 16 == 0));
+  const auto run = p->io ? rotary<uint16_t> : rotary<float>;
+  return ops::hip_status(run(a, (long long)p->B * p->T, p->interleaved, wide, (hipStream_t)stream), "rotary launch");
+}
+
+int sffft_rotary_table(int positions, int R, double base, int scaling, double factor, int trained, double magnitude,
+                       float* table) {
+  if (positions < 1 || R < 2 || R % 2 || !(base > 0) || !std::isfinite(base) || scaling < SFFFT_ROTARY_NONE ||
+      scaling > SFFFT_ROTARY_PARTS || !(factor > 0) || !std::isfinite(factor) || !std::isfinite(magnitude) || !table ||
+      (scaling == SFFFT_ROTARY_PARTS && trained < 1))
+    return SFFFT_EINVAL;
+  if (scaling == SFFFT_ROTARY_STRETCHED && R > 2) base *= std::pow(factor, (double)R / (R - 2));
+  for (int i = 0; i < R / 2; i++) {
+    double f = std::pow(base, -2.0 * i / R);
+    if (scaling == SFFFT_ROTARY_LINEAR) f /= factor;
+    if (scaling == SFFFT_ROTARY_PARTS) {
+      const double turns = trained * f / (2 * M_PI), keep = std::min(1.0, std::max(0.0, (turns - 1) / 31));
+      f = f * keep + f / factor * (1 - keep);
+    }
+    for (int n = 0; n < positions; n++) {
+      table[(size_t)n * R + i] = (float)(magnitude * std::cos(n * f));
+      table[(size_t)n * R + R / 2 + i] = (float)(magnitude * std::sin(n * f));
+    }
+  }
+  return SFFFT_OK;
+}
+
+int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, const void* gate, const float* w_pre,
+                        const float* w_post, const float* scale, void* r, void* h, void* stream) {
+  if (!valid_norm(p) || !x || !h || !w_pre || (y != nullptr) != (r != nullptr) || (!y && (gate || w_post || scale)))
+    return SFFFT_EINVAL;
+  const int elem = p->io ? 2 : 4;
+  const long long gates = p->rows / p->gate_rows;
+  const size_t vec = (size_t)p->C * 4, nx = row_bytes(p, p->x, p->rows), ny = y ? row_bytes(p, p->y, p->rows) : 1;
+  const size_t ng = gate ? row_bytes(p, p->gate, gates) : 1, no = (size_t)p->rows * p->C * elem;
+  if (!nx || !ny || !ng) return SFFFT_EINVAL;
+  const Span in[] = {{x, nx}, {y, ny}, {gate, ng}, {w_pre, vec}, {w_post, vec}, {scale, vec}};
+  const Span out[] = {{r, no}, {h, no}};
+  for (int i = 0; i < 6; i++)
+    if (!ops::aligned(in[i].p, i < 3 ? elem : 4)) return SFFFT_EINVAL;
+  if (!ops::aligned(r, elem) || !ops::aligned(h, elem) || !apart(in, 6, out, 2)) return SFFFT_EINVAL;
+  const long long strides[] = {p->x, y ? p->y : 0, gate ? p->gate : 0};
+  const Span act[] = {{x, 0}, {y, 0}, {gate, 0}, {r, 0}, {h, 0}};
+  bool wide = wide_rows(p, act, 5, strides, 3);
+  for (const float* w : {w_pre, w_post, scale}) wide = wide && ops::aligned(w, 16);
+  const RowShape s = row_shape(p->C, wide);
+  const Parts q = parts_of(p, s, false);
+  if (q.nparts > INT_MAX) return SFFFT_EINVAL;
+  bn::Args a = {};
+  a.x = x, a.y = y, a.gate = gate, a.sx = p->x, a.sy = p->y, a.sg = p->gate;
+  a.wq = w_pre, a.wp = w_post, a.sc = scale, a.r = r, a.h = h;
+  a.rows = p->rows, a.gate_rows = p->gate_rows, a.C = p->C, a.act = p->act, a.eps = p->eps, a.part_rows = q.part_rows;
+  const auto run = p->io ? norm<uint16_t> : norm<float>;
+  return ops::hip_status(run(a, s, y != nullptr, false, dim3((unsigned)q.nparts), (hipStream_t)stream),
+                         "block norm launch");
+}
+
+// The parts of the forms with and without wide loads differ in nothing: row_shape's lanes do not depend on it.
+size_t sffft_blocknorm_work_bytes(const sffft_blocknorm* p, int has_y, int has_gate) {
+  if (!valid_norm(p)) return 0;
+  const bool shared = has_gate && p->gate_rows > 1;
+  const Parts q = parts_of(p, row_shape(p->C, true), shared);
+  return (size_t)(has_y ? shared ? 4 : 3 : 1) * q.nparts * p->C * 4;
+}
+
+int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, const void* gate, const float* w_pre,
+                        const float* w_post, const float* scale, const void* gr, const void* gh, void* dx, void* dy,
+                        void* dgate, float* dw_pre, float* dw_post, float* dscale, void* work, size_t work_bytes,
+                        void* stream) {
+  if (!valid_norm(p) || !x || !w_pre || !dx || !dw_pre || (!gr && !gh) || (y != nullptr) != (dy != nullptr) ||
+      (gate != nullptr) != (dgate != nullptr) || (w_post != nullptr) != (dw_post != nullptr) ||
+      (scale != nullptr) != (dscale != nullptr) || (!y && (gate || w_post || scale)))
+    return SFFFT_EINVAL;
+  const int elem = p->io ? 2 : 4;
+  const bool shared = gate && p->gate_rows > 1;
+  const long long gates = p->rows / p->gate_rows;
+  const size_t vec = (size_t)p->C * 4, no = (size_t)p->rows * p->C * elem;
+  const size_t nx = row_bytes(p, p->x, p->rows), ny = y ? row_bytes(p, p->y, p->rows) : 1;
+  const size_t ng = gate ? row_bytes(p, p->gate, gates) : 1, nr = gr ? row_bytes(p, p->gr, p->rows) : 1;
+  const size_t nh = gh ? row_bytes(p, p->gh, p->rows) : 1, need = sffft_blocknorm_work_bytes(p, y != nullptr, gate != nullptr);
+  if (!nx || !ny || !ng || !nr || !nh || !work || work_bytes < need || !ops::aligned(work, 16)) return SFFFT_EINVAL;
+  const Span in[] = {{x, nx}, {y, ny}, {gate, ng}, {gr, nr}, {gh, nh}, {w_pre, vec}, {w_post, vec}, {scale, vec}};
+  const Span out[] = {{dx, no}, {dy, no}, {dgate, (size_t)gates * p->C * elem}, {dw_pre, vec}, {dw_post, vec},
+                      {dscale, vec}, {work, need}};
+  for (int i = 0; i < 8; i++)
+    if (!ops::aligned(in[i].p, i < 5 ? elem : 4)) return SFFFT_EINVAL;
+  for (int i = 0; i < 6; i++)
+    if (!ops::aligned(out[i].p, i < 3 ? elem : 4)) return SFFFT_EINVAL;
+  if (!apart(in, 8, out, 7)) return SFFFT_EINVAL;
+  const long long strides[] = {p->x, y ? p->y : 0, gate ? p->gate : 0, gr ? p->gr : 0, gh ? p->gh : 0};
+  const Span act[] = {{x, 0}, {y, 0}, {gate, 0}, {gr, 0}, {gh, 0}, {dx, 0}, {dy, 0}, {dgate, 0}};
+  bool wide = wide_rows(p, act, 8, strides, 5);
+  for (const float* w : {w_pre, w_post, scale}) wide = wide && ops::aligned(w, 16);
+  const RowShape s = row_shape(p->C, wide);
+  const Parts q = parts_of(p, s, shared);
+  if (q.nparts > INT_MAX) return SFFFT_EINVAL;
+  bn::Args a = {};
+  a.x = x, a.y = y, a.gate = gate, a.gr = gr, a.gh = gh;
+  a.sx = p->x, a.sy = p->y, a.sg = p->gate, a.sgr = p->gr, a.sgh = p->gh;
+  a.wq = w_pre, a.wp = w_post, a.sc = scale, a.dx = dx, a.dy = dy, a.dgate = dgate;
+  a.parts = static_cast<float*>(work), a.rows = p->rows, a.gate_rows = gate ? p->gate_rows : 1;
+  a.block_rows = q.block_rows, a.C = p->C, a.act = p->act, a.part_rows = q.part_rows, a.parts_per_block = q.per_block;
+  a.nparts = q.nparts, a.eps = p->eps;
+  hipStream_t st = (hipStream_t)stream;
+  const auto run = p->io ? norm<uint16_t> : norm<float>;
+  hipError_t err = run(a, s, y != nullptr, true, dim3((unsigned)q.nparts), st);
+  const unsigned tiles = (unsigned)((p->C + 63) / 64);
+  float* const sums[] = {dw_pre, dw_post, dscale};
+  for (int i = 0; i < 3 && err == hipSuccess; i++)
+    if (sums[i]) {
+      hipLaunchKernelGGL(bn::sum_kernel<float>, dim3(tiles), dim3(256), 0, st, a.parts + (size_t)i * q.nparts * p->C,
+                         sums[i], p->C, (int)q.nparts);
+      err = hipGetLastError();
+    }
+  if (err == hipSuccess && shared) {
+    const float* parts = a.parts + (size_t)3 * q.nparts * p->C;
+    const dim3 grid((unsigned)(tiles * q.blocks));
+    if (p->io)
+      hipLaunchKernelGGL(bn::sum_kernel<uint16_t>, grid, dim3(256), 0, st, parts, static_cast<uint16_t*>(dgate), p->C,
+                         q.per_block);
+    else
+      hipLaunchKernelGGL(bn::sum_kernel<float>, grid, dim3(256), 0, st, parts, static_cast<float*>(dgate), p->C,
+                         q.per_block);
+    err = hipGetLastError();
+  }
+  return ops::hip_status(err, "block norm gradient launch");
+}
+
+const char* sffft_ops_last_error(void) { return ops::g_last_error; }
+
+}  // extern "C"

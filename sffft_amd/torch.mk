@@ -1,6 +1,6 @@
-# Builds libsffft_torch.so, the PyTorch operators (csrc/torch_ops.cpp): host code only, compiled
-# with the host compiler against the installed torch's headers and libraries, linked to
-# libsffft.so (which the main Makefile builds). Kept apart from the kernel build so that the
+# Builds libsffft_torch.so, the PyTorch operators (csrc/torch_ops.cpp, csrc/torch_mixers.cpp): host
+# code only, compiled with the host compiler against the installed torch's headers and libraries,
+# linked to libsffft.so (which the main Makefile builds) and libsffft_ops.so (ops.mk). Kept apart from the kernel build so that the
 # kernel recipe, and so the kernel-source stamp of the profile summaries, does not depend on it.
 #   make -C sffft_amd -f torch.mk
 ROCM ?= /opt/rocm
@@ -16,9 +16,15 @@ TORCH_FLAGS = -O2 -std=c++17 -fPIC -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -D_GLIBCXX_
 .PHONY: all clean
 all: libsffft_torch.so
 
-libsffft_torch.so: csrc/torch_ops.cpp ../include/sffft.h libsffft.so
-	$(CXX) $(TORCH_FLAGS) -shared -o $@ $< -L. -lsffft -L$(TORCH_DIR)/lib -lc10 -lc10_hip -ltorch_cpu -ltorch \
+_build/torch_ops.o: ../include/sffft.h
+_build/torch_mixers.o: ../include/sffft.h ../include/sffft_ops.h
+_build/torch_%.o: csrc/torch_%.cpp
+	@mkdir -p _build
+	$(CXX) $(TORCH_FLAGS) -c -o $@ $<
+
+libsffft_torch.so: _build/torch_ops.o _build/torch_mixers.o libsffft.so libsffft_ops.so
+	$(CXX) -shared -o $@ _build/torch_ops.o _build/torch_mixers.o -L. -lsffft -lsffft_ops -L$(TORCH_DIR)/lib -lc10 -lc10_hip -ltorch_cpu -ltorch \
 	  -Wl,-rpath,'$$ORIGIN' -Wl,-rpath,$(TORCH_DIR)/lib
 
 clean:
-	rm -f libsffft_torch.so
+	rm -f _build/torch_*.o libsffft_torch.so

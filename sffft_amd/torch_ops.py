@@ -26,6 +26,12 @@ Gradients:
   gradient is the batch-summed correlation dk[h, j] = sum_b sum_{n >= j} dy[b, h, n] u[b, h, n - j]
   (``torch.ops.sffft.filter_grad``).
 - ``spectrum`` itself has no gradient and raises if its filter requires grad.
+
+The operators beside the convolution (``csrc/torch_mixers.cpp``, over libsffft_ops.so) are here too:
+``torch.ops.sffft.linear_attention`` / ``linear_attention_step`` (linear attention with a decay for
+each head), ``rotary`` / ``rotary_`` (with tables from ``sffft_amd.mixers.rotary_table``),
+``block_norm`` and ``pre_norm``. linear_attention, rotary and the norms are differentiable (once;
+rotary any number of times); decays and tables are constants.
 """
 from __future__ import annotations
 
@@ -84,6 +90,73 @@ def _longconv_fake(u, k, kf, plan):
 def _filter_grad_fake(u, dy):
     torch._check(u.dim() == 3 and dy.shape == u.shape, lambda: "u and dy must be [B, H, L]")
     return u.new_empty((u.shape[1], u.shape[2]), dtype=torch.float32)
+
+
+@torch.library.register_fake("sffft::linear_attention")
+def _linear_attention_fake(q, k, v, log_decay, scale, initial_state=None, lengths=None):
+    torch._check(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, lambda: "q, k, v must be [B, T, heads, channels]")
+    torch._check(q.dtype in (torch.float32, torch.bfloat16) and k.dtype == q.dtype and v.dtype == q.dtype,
+                 lambda: "q, k, v must all be float32 or all bfloat16")
+    torch._check(k.shape[:2] == q.shape[:2] and v.shape[:3] == k.shape[:3] and k.shape[3] == q.shape[3]
+                 and q.shape[2] % k.shape[2] == 0, lambda: "k and v must be the keys and values of q's tokens")
+    torch._check(q.shape[3] % 8 == 0 and v.shape[3] % 8 == 0 and q.shape[3] <= 128 and v.shape[3] <= 128,
+                 lambda: "head channels must be multiples of 8 up to 128")
+    torch._check(log_decay.shape == q.shape[2:3], lambda: "log_decay must be [H]")
+    B, T, H, Dk = q.shape
+    return q.new_empty((B, T, H, v.shape[3])), q.new_empty((B, H, Dk, v.shape[3]), dtype=torch.float32)
+
+
+@torch.library.register_fake("sffft::linear_attention_backward")
+def _linear_attention_backward_fake(q, k, v, log_decay, scale, initial_state, lengths, grad_o, grad_state):
+    B, T, H, Dk = q.shape
+    return (q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape),
+            q.new_empty((B, H, Dk, v.shape[3]), dtype=torch.float32))
+
+
+@torch.library.register_fake("sffft::linear_attention_step")
+def _linear_attention_step_fake(q, k, v, log_decay, state, scale, slots=None):
+    torch._check(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, lambda: "q, k, v must be [B, heads, channels]")
+    torch._check(k.shape[0] == q.shape[0] and v.shape[:2] == k.shape[:2] and k.shape[2] == q.shape[2]
+                 and q.shape[1] % k.shape[1] == 0, lambda: "k and v must be the keys and values of q's tokens")
+    torch._check(state.dim() == 4 and state.shape[1:] == (q.shape[1], q.shape[2], v.shape[2]),
+                 lambda: "the state must be [slots, H, Dk, Dv]")
+    return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
+
+
+@torch.library.register_fake("sffft::rotary")
+def _rotary_fake(q, k, table, positions=None, interleaved=False, inverse=False):
+    torch._check(q.dim() == 4 and k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == q.shape[3],
+                 lambda: "q and k must be [B, T, H, D] and [B, T, Hk, D]")
+    torch._check(table.dim() == 2 and table.shape[1] % 2 == 0 and table.shape[1] <= q.shape[3],
+                 lambda: "table must be [positions, R], R even and at most D")
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.register_fake("sffft::rotary_")
+def _rotary_inplace_fake(q, k, table, positions=None, interleaved=False):
+    return None
+
+
+@torch.library.register_fake("sffft::block_norm")
+def _block_norm_fake(x, y, w_pre, w_post=None, gate=None, scale=None, activation="none", eps=1e-6):
+    torch._check(y.shape == x.shape and y.dtype == x.dtype, lambda: "y must have x's shape and type")
+    torch._check(w_pre.shape == x.shape[-1:], lambda: "w_pre must be [C]")
+    torch._check(activation in ("none", "sigmoid", "silu"), lambda: "activation must be none, sigmoid or silu")
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+@torch.library.register_fake("sffft::pre_norm")
+def _pre_norm_fake(x, w, eps=1e-6):
+    torch._check(w.shape == x.shape[-1:], lambda: "w must be [C]")
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("sffft::block_norm_backward")
+def _block_norm_backward_fake(grad_r, grad_h, x, y, w_pre, w_post, gate, scale, activation, eps):
+    def like(t):
+        return x.new_empty((0,), dtype=torch.float32) if t is None else t.new_empty(t.shape)
+
+    return like(x), like(y), like(gate), like(w_pre), like(w_post), like(scale)
 
 
 def filter_grad(u: torch.Tensor, dy: torch.Tensor) -> torch.Tensor:
