@@ -1,4 +1,5 @@
 // Launches and C ABI of linear attention (linattn.hpp).
+#include <algorithm>
 #include <climits>
 
 #include "linattn.hpp"
@@ -31,9 +32,37 @@ bool valid_input(const void* x, const long long s[3], const sffft_linattn* p, in
 
 Operand operand(const void* x, const long long s[3], int div) { return {x, s[0], s[1], s[2], div}; }
 
-template <class T>
-hipError_t recur(const March& m, const Shape& s, hipStream_t st) {
-  hipLaunchKernelGGL(la::recur_kernel<T>, dim3((unsigned)(s.B * s.H * ((m.V + 15) / 16))), dim3(64), 0, st, m, s);
+// How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march.
+struct Cut {
+  int nseg, seg;
+};
+Cut cut_of(const sffft_linattn* p, int marches) {
+  const int C = p->io ? la::chunk_of<uint16_t>() : la::chunk_of<float>(), D = std::max(p->Dk, p->Dv);
+  const int chunks = (p->T + C - 1) / C, fill = D > 64 ? 512 : 1024;
+  const long long heads = (long long)p->B * p->H * marches;
+  const int want = (int)std::min<long long>(chunks, std::max<long long>(1, fill / heads));
+  const int per = (chunks + want - 1) / want;
+  return {(chunks + per - 1) / per, per * C};
+}
+
+template <class T, int KT, int VT, bool OUT>
+hipError_t launch(la::Launch& L, hipStream_t st) {
+  L.vtiles = 1;
+  for (int i = 0; i < L.nm; i++) L.vtiles = std::max(L.vtiles, (L.m[i].V + VT - 1) / VT);
+  const int units = L.s.B * L.s.H * L.nseg;
+  hipLaunchKernelGGL((la::march_kernel<T, KT, VT, OUT>), dim3((unsigned)((units + 7) / 8 * 8 * L.nm * L.vtiles)),
+                     dim3(256), 0, st, L);
+  return hipGetLastError();
+}
+// D: the most channels of any operand
+template <class T, bool OUT>
+hipError_t march(la::Launch L, int D, hipStream_t st) {
+  constexpr int VT = sizeof(T) == 4 ? 64 : 128;  // fp32: the planes of 128 columns leave no room for a second workgroup
+  return D > 64 ? launch<T, 128, VT, OUT>(L, st) : launch<T, 64, 64, OUT>(L, st);
+}
+hipError_t scan(const la::ScanLaunch& L, int n, hipStream_t st) {
+  const unsigned tiles = (unsigned)((L.c[0].n + 1023) / 1024);
+  hipLaunchKernelGGL(la::scan_kernel, dim3((unsigned)(L.s.B * L.s.H) * tiles, (unsigned)n), dim3(256), 0, st, L);
   return hipGetLastError();
 }
 
@@ -44,36 +73,63 @@ hipError_t head_sum(const float* in, void* out, long long n, int D, int G, hipSt
   return hipGetLastError();
 }
 
-template <class T>
-hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const void* v, const Shape& s,
-                   const float* s0, void* o, float* s1, hipStream_t st) {
-  const int G = p->H / p->Hk;
-  return recur<T>({operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, s1, p->Dk, p->Dv, p->Dv, 1, 0,
-                   0, p->scale, p->scale, 1.f},
-                  s, st);
+// The segments' states
+size_t state_bytes(const sffft_linattn* p, const Cut& c) {
+  return c.nseg == 1 ? 0 : (size_t)p->B * p->H * c.nseg * p->Dk * p->Dv * 4;
 }
-
 // dk and dv of heads that are shared, for each query head, before their sum
 size_t shared_bytes(const sffft_linattn* p) {
   return p->H == p->Hk ? 0 : (size_t)p->B * p->T * p->H * (p->Dk + p->Dv) * 4;
 }
 
 template <class T>
+hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const void* v, const Shape& s,
+                   const float* s0, void* o, float* s1, float* work, hipStream_t st) {
+  const int G = p->H / p->Hk, D = std::max(p->Dk, p->Dv);
+  const Cut cut = cut_of(p, 1);
+  const long long n = (long long)p->Dk * p->Dv;
+  March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, n, 0, s1, n, 0,
+             p->Dk, p->Dv, p->Dv, 1, 0, 0, p->scale, p->scale, 1.f};
+  la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1};
+  if (cut.nseg > 1) {
+    L.m[0].s0 = nullptr, L.m[0].s1 = work, L.m[0].s1_bh = n * cut.nseg, L.m[0].s1_seg = n;
+    hipError_t e = march<T, false>(L, D, st);
+    if (e == hipSuccess) e = scan({{{work, s0, s1, (int)n, 0}}, s, cut.nseg, cut.seg}, 1, st);
+    if (e != hipSuccess) return e;
+    L.m[0] = m, L.m[0].s0 = work, L.m[0].s0_bh = n * cut.nseg, L.m[0].s0_seg = n, L.m[0].s1 = nullptr;
+  }
+  return march<T, true>(L, D, st);
+}
+
+template <class T>
 hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const void* v, const void* go,
                     const Shape& s, const float* s0, const float* ds1, void* dq, void* dk, void* dv, float* ds0,
                     float* work, hipStream_t st) {
-  const int G = p->H / p->Hk;
+  const int G = p->H / p->Hk, D = std::max(p->Dk, p->Dv), Dk = p->Dk, Dv = p->Dv;
   const Operand Q = operand(q, p->q, 1), K = operand(k, p->k, G), V = operand(v, p->v, G), O = operand(go, p->go, 1);
   const size_t rows = (size_t)p->B * p->T;
-  float *wk = work, *wv = work + rows * p->H * p->Dk;
+  const Cut cut = cut_of(p, 3);
+  const long long n = (long long)Dk * Dv, ns = cut.nseg > 1 ? n * cut.nseg : n, nz = cut.nseg > 1 ? n : 0;
+  float *ws = work, *wd = ws + state_bytes(p, cut) / 4, *wk = wd + state_bytes(p, cut) / 4, *wv = wk + rows * p->H * Dk;
   const float c = p->scale;
-  hipError_t e = recur<T>({O, V, K, dq, s0, nullptr, p->Dv, p->Dk, 1, p->Dv, 0, 0, c, c, 1.f}, s, st);
-  if (e == hipSuccess)
-    e = recur<T>({K, Q, O, G > 1 ? wv : dv, ds1, ds0, p->Dk, p->Dv, p->Dv, 1, 1, G > 1, c, 1.f, c}, s, st);
-  if (e == hipSuccess)
-    e = recur<T>({V, O, Q, G > 1 ? wk : dk, ds1, nullptr, p->Dv, p->Dk, 1, p->Dv, 1, G > 1, c, 1.f, c}, s, st);
-  if (e == hipSuccess && G > 1) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * p->Dk, p->Dk, G, st);
-  if (e == hipSuccess && G > 1) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * p->Dv, p->Dv, G, st);
+  la::Launch L = {{}, s, 3, cut.nseg, cut.seg, 1};
+  hipError_t e = hipSuccess;
+  if (cut.nseg > 1) {
+    L.nm = 2;
+    L.m[0] = {Q, K, V, nullptr, nullptr, 0, 0, ws, ns, n, Dk, Dv, Dv, 1, 0, 0, c, c, 1.f};
+    L.m[1] = {K, Q, O, nullptr, nullptr, 0, 0, wd, ns, n, Dk, Dv, Dv, 1, 1, 0, c, 1.f, c};
+    e = march<T, false>(L, D, st);
+    if (e == hipSuccess)
+      e = scan({{{ws, s0, nullptr, (int)n, 0}, {wd, ds1, ds0, (int)n, 1}}, s, cut.nseg, cut.seg}, 2, st);
+    if (e != hipSuccess) return e;
+    s0 = ws, ds1 = wd, ds0 = nullptr, L.nm = 3;
+  }
+  L.m[0] = {O, V, K, dq, s0, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 0, 0, c, c, 1.f};
+  L.m[1] = {K, Q, O, G > 1 ? wv : dv, ds1, ns, nz, ds0, n, 0, Dk, Dv, Dv, 1, 1, G > 1, c, 1.f, c};
+  L.m[2] = {V, O, Q, G > 1 ? wk : dk, ds1, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 1, G > 1, c, 1.f, c};
+  e = march<T, true>(L, D, st);
+  if (e == hipSuccess && G > 1) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * Dk, Dk, G, st);
+  if (e == hipSuccess && G > 1) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * Dv, Dv, G, st);
   return e;
 }
 
@@ -86,7 +142,7 @@ extern "C" {
 
 size_t sffft_linattn_work_bytes(const sffft_linattn* p, int backward) {
   if (!valid_shape(p)) return 0;
-  return backward ? shared_bytes(p) : 0;
+  return backward ? 2 * state_bytes(p, cut_of(p, 3)) + shared_bytes(p) : state_bytes(p, cut_of(p, 1));
 }
 
 int sffft_linattn_fwd(const sffft_linattn* p, const void* q, const void* k, const void* v, const float* log_decay,
@@ -113,7 +169,7 @@ int sffft_linattn_fwd(const sffft_linattn* p, const void* q, const void* k, cons
     if (need && ops::overlap(work, need, in[i], len[i])) return SFFFT_EINVAL;
   const Shape s = {p->B, p->T, p->H, log_decay, lengths};
   const auto run = p->io ? forward<uint16_t> : forward<float>;
-  return ops::hip_status(run(p, q, k, v, s, initial_state, o, final_state, (hipStream_t)stream),
+  return ops::hip_status(run(p, q, k, v, s, initial_state, o, final_state, static_cast<float*>(work), (hipStream_t)stream),
                          "linear attention launch");
 }
 

@@ -1,15 +1,34 @@
 // Linear attention with a decay for each head. Forward and all three gradients are one recurrence
 // over a state X [K][V] with operands a, b (K channels) and c (V channels):
 //
-//   out_i = sum_{j <= i} g^(i-j) (a_i . b_j) c_j + g^(i+1) X0^T a_i        (REV: j >= i, g^(j-i))
+//   out_i = sum_{j <= i} g^(i-j) (a_i . b_j) c_j + g^(i+1) X0^T a_i        (rev: j >= i, g^(j-i))
 //
 //   o  : a = q,  b = k,  c = v            dv : a = k, b = q,  c = do, reversed in time
 //   dq : a = do, b = v,  c = k, X = S^T   dk : a = v, b = do, c = q,  reversed, X = dS^T
+//
+// A workgroup marches over the tokens of one head in chunks of 64 (fp32: 32) with the state in its
+// registers. For a chunk of n tokens entered with X:
+//   P_ij = g^(i-j) (a_i . b_j) for j <= i,   out = P c + g^(i+1) a X,   X' = g^n X + sum_j g^(n-1-j) b_j c_j^T
+// all four products on MFMA; every decay is a power of g not above 1, so nothing overflows however fast a head
+// forgets. Where the heads alone do not fill the chip the tokens are cut into segments: a first launch
+// sums each segment's own state, a second carries the states over the segments, and the march starts every
+// segment with its own.
+//
+// Operands in 16 bits: bf16 inputs are exact; P and the entering state are rounded to bf16 where they
+// are operands of a product that is rounded to bf16 itself in the end (their errors are of that
+// rounding's size). The state is fp32 and so are the decayed c_j that are added to it: they are split
+// into three bf16 parts (8 bits each, 24 together), one product each. fp32 inputs are split so too, and
+// every product of two split operands is the six partial products above 2^-24.
 #pragma once
 #include "opsio.hpp"
 
 namespace sffft {
 namespace la {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16;
 
 // One operand: element strides of (batch, token, head); head h of the march reads head h / div.
 struct Operand {
@@ -18,15 +37,17 @@ struct Operand {
   int div;
 };
 
-// One march: state element (kk, vv) of (b, h) is at s[(b * H + h) * K * V + kk * sk + vv * sv].
-// The update adds w b c^T; the products with the entering state take x, those within the march p.
-// Forward, the state enters before a token's own update (a_0 sees g X0); reversed, it holds all from the
-// token on (the first one sees X0 undecayed, and the update includes the decay of the step).
+// One march. State element (kk, vv) of (b, h) in segment z is at s[(b * H + h) * s_bh + z * s_seg + kk * sk
+// + vv * sv]. The update adds w b c^T; the products with the entering state take x, those within
+// the march p. Forward, the state enters before a token's own update (a_0 sees g X0); reversed, it holds all
+// from the token on (the first one sees X0 undecayed, and the update includes the decay of the step).
 struct March {
   Operand a, b, c;
   void* out;  // [B][T][H][V], in the operands' type, or fp32 if out_f32
   const float* s0;
+  long long s0_bh, s0_seg;
   float* s1;
+  long long s1_bh, s1_seg;
   int K, V, sk, sv;
   int rev, out_f32;
   float p, x, w;
@@ -38,6 +59,13 @@ struct Shape {
   const int* lengths;
 };
 
+// A launch: nm marches over B * H heads, nseg segments of seg tokens, vtiles tiles of the V channels.
+struct Launch {
+  March m[3];
+  Shape s;
+  int nm, nseg, seg, vtiles;
+};
+
 constexpr float LOG2E = 1.44269504088896340736f;
 
 // log2 of the decay; -inf becomes a finite value whose powers are 0, so that the zeroth is 1
@@ -46,58 +74,411 @@ __device__ __forceinline__ int valid_tokens(const Shape& s, int b) {
   return s.lengths ? min(max(s.lengths[b], 0), s.T) : s.T;
 }
 
-// The recurrence token by token: one wavefront holds 16 columns of the state, lane (r, c) the rows
-// r, r + 4, ... of column c.
-template <class T>
-__global__ __launch_bounds__(64) void recur_kernel(March m, Shape s) {
-  constexpr int ROWS = 32;
-  const int tiles = (m.V + 15) / 16, bh = blockIdx.x / tiles, h = bh % s.H, b = bh / s.H;
-  const int r = threadIdx.x >> 4, col = (blockIdx.x - bh * tiles) * 16 + (threadIdx.x & 15);
-  const bool in = col < m.V;
-  const float g = exp2f(decay_log2(s.log_decay, h));
-  const int n = valid_tokens(s, b);
-  const T* a = static_cast<const T*>(m.a.p) + b * m.a.sb + (h / m.a.div) * m.a.sh;
-  const T* bb = static_cast<const T*>(m.b.p) + b * m.b.sb + (h / m.b.div) * m.b.sh;
-  const T* c = static_cast<const T*>(m.c.p) + b * m.c.sb + (h / m.c.div) * m.c.sh;
-  const long long at = (long long)bh * m.K * m.V + (long long)col * m.sv;
-  float x[ROWS];
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// x = h + m + l exactly, 8 bits each, truncated; two values to a dword of each plane
+__device__ __forceinline__ void split2(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  const uint32_t xh = __float_as_uint(x) & 0xffff0000u, yh = __float_as_uint(y) & 0xffff0000u;
+  const float xr = x - __uint_as_float(xh), yr = y - __uint_as_float(yh);
+  const uint32_t xm = __float_as_uint(xr) & 0xffff0000u, ym = __float_as_uint(yr) & 0xffff0000u;
+  const float xl = xr - __uint_as_float(xm), yl = yr - __uint_as_float(ym);
+  h = __builtin_amdgcn_perm(yh, xh, 0x07060302);
+  m = __builtin_amdgcn_perm(ym, xm, 0x07060302);
+  l = __builtin_amdgcn_perm(__float_as_uint(yl), __float_as_uint(xl), 0x07060302);
+}
+
+// NS planes of one operand fragment
+template <int NS>
+struct Frag {
+  bf16x8 p[NS];
+};
+// d += a b, the products of planes that are not below the last one's bits
+template <int NA, int NB>
+__device__ __forceinline__ void product(const Frag<NA>& a, const Frag<NB>& b, f32x4& d) {
+  constexpr int LAST = (NA > NB ? NA : NB) - 1;
 #pragma unroll
-  for (int i = 0; i < ROWS; i++) {
-    const int kk = r + 4 * i;
-    x[i] = in && kk < m.K && m.s0 ? m.s0[at + (long long)kk * m.sk] : 0.f;
+  for (int s = LAST; s >= 0; s--)
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+      if (s - i >= 0 && s - i < NB) d = mfma(a.p[i], b.p[s - i], d);
+}
+template <int NS>
+__device__ __forceinline__ Frag<NS> split8(const float (&x)[8]) {
+  Frag<NS> f;
+  if constexpr (NS == 1) {
+    const uint4 v = make_uint4(ops::pack_bf16(x[0], x[1]), ops::pack_bf16(x[2], x[3]), ops::pack_bf16(x[4], x[5]),
+                               ops::pack_bf16(x[6], x[7]));
+    f.p[0] = __builtin_bit_cast(bf16x8, v);
+  } else {
+    uint32_t h[4], m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], m[i], l[i]);
+    f.p[0] = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
+    f.p[1] = __builtin_bit_cast(bf16x8, make_uint4(m[0], m[1], m[2], m[3]));
+    f.p[2] = __builtin_bit_cast(bf16x8, make_uint4(l[0], l[1], l[2], l[3]));
   }
-  for (int i = 0; i < s.T; i++) {
-    const int t = m.rev ? s.T - 1 - i : i;
-    float o = 0.f;
-    if (t < n) {
-      const float cv = in ? ops::to_f32(c[t * m.c.st + col]) : 0.f;
-      // reversed, the state's own scale is in it already; what enters and what is added are equal there
-      const float up = m.rev ? m.w : 1.f;
+  return f;
+}
+
+// Row-major [C][L] tiles of 16 bits in LDS, NS planes. Rows are padded by 32 bytes: the transposing reads below
+// touch 8 rows of 32 bytes at a time, on 64 different banks.
+template <int NS, int C, int L>
+struct Tile {
+  u16 v[NS][C][L];
+
+  // operand whose index is the row: lane (g, i) holds channels at..at+7 of row r0 + i, at = c0 + 8 g
+  __device__ __forceinline__ Frag<NS> rows(int r0, int c0, int i, int g) const {
+    Frag<NS> f;
 #pragma unroll
-      for (int e = 0; e < ROWS; e++) {
-        const int kk = r + 4 * e;
-        if (kk < m.K) {
-          if (!m.rev || t < n - 1) x[e] *= g;
-          x[e] += up * ops::to_f32(bb[t * m.b.st + kk]) * cv;
-          o += ops::to_f32(a[t * m.a.st + kk]) * x[e];
+    for (int p = 0; p < NS; p++) f.p[p] = *reinterpret_cast<const bf16x8*>(&v[p][r0 + i][c0 + 8 * g]);
+    return f;
+  }
+  // the same with the channels in the order of an accumulator's rows: c0 + 4 g .. + 3 and c0 + 16 + 4 g .. + 3
+  __device__ __forceinline__ Frag<NS> rows_acc(int r0, int c0, int i, int g) const {
+    Frag<NS> f;
+#pragma unroll
+    for (int p = 0; p < NS; p++) {
+      const uint2 a = *reinterpret_cast<const uint2*>(&v[p][r0 + i][c0 + 4 * g]);
+      const uint2 b = *reinterpret_cast<const uint2*>(&v[p][r0 + i][c0 + 16 + 4 * g]);
+      f.p[p] = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
+    }
+    return f;
+  }
+  // operand whose index is the channel: lane (g, i) holds rows r0 + 4 g .. + 3 and r0 + 16 + 4 g .. + 3 of
+  // channel c0 + i. A transposing read takes 4 rows of 16 channels for each 16 lanes: lane i points at
+  // row i / 4, channels 4 (i % 4).., and receives channel i of the four rows.
+  __device__ __forceinline__ Frag<NS> cols(int r0, int c0, int i, int g) const {
+    Frag<NS> f;
+#pragma unroll
+    for (int p = 0; p < NS; p++) {
+      const u16* q = &v[p][r0 + 4 * g + (i >> 2)][c0 + 4 * (i & 3)];
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q);
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 16 * L));
+      const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+      f.p[p] = __builtin_bit_cast(bf16x8, make_uint4(x.x, x.y, y.x, y.y));
+    }
+    return f;
+  }
+};
+
+// A chunk's rows of one operand on their way from memory to LDS: 16 bytes a piece, rows from n on and channels
+// from D on are zero and not read.
+template <class T, int C, int DT>
+struct Stage {
+  static constexpr int E = 16 / sizeof(T), PER = DT / E, N = C * PER / 256;
+  uint4 v[N];
+  __device__ __forceinline__ void load(const T* p, long long st, int n, int D) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int piece = threadIdx.x + 256 * i, row = piece / PER, col = piece % PER * E;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (row < n && col < D) v[i] = *reinterpret_cast<const uint4*>(p + row * st + col);
+    }
+  }
+  template <int NS, int L>
+  __device__ __forceinline__ void store(Tile<NS, C, L>& t) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int piece = threadIdx.x + 256 * i, row = piece / PER, col = piece % PER * E;
+      if constexpr (NS == 1) {
+        *reinterpret_cast<uint4*>(&t.v[0][row][col]) = v[i];
+      } else {
+        uint2 h, m, l;
+        split2(__uint_as_float(v[i].x), __uint_as_float(v[i].y), h.x, m.x, l.x);
+        split2(__uint_as_float(v[i].z), __uint_as_float(v[i].w), h.y, m.y, l.y);
+        *reinterpret_cast<uint2*>(&t.v[0][row][col]) = h;
+        *reinterpret_cast<uint2*>(&t.v[1][row][col]) = m;
+        *reinterpret_cast<uint2*>(&t.v[2][row][col]) = l;
+      }
+    }
+  }
+};
+
+template <class T>
+constexpr int chunk_of() { return sizeof(T) == 4 ? 32 : 64; }
+
+// Four wavefronts; wavefront w holds the columns vv = v0 + w VT/4 .. of the state, in the layout of an
+// accumulator (row kk = 16 a + 4 g + r, column lane % 16), which is an operand's too when the other operand
+// takes the same order of channels (rows_acc). With !OUT only the state is made.
+template <class T, int KT, int VT, bool OUT>
+__global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
+  constexpr int NS = sizeof(T) == 4 ? 3 : 1, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, VW = VT / 64;
+  constexpr int TILES = MT * (MT + 1) / 2, NP = (TILES + 3) / 4;
+  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, KT + 16> ta;
+  __shared__ __attribute__((aligned(16))) Tile<NS, C, KT + 16> tb;
+  __shared__ __attribute__((aligned(16))) Tile<NS, C, VT + 16> tc;
+  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, C + 8> tp;
+
+  // Workgroups go to the 8 XCDs in turn; the marches and V tiles of one head and segment, which read the same
+  // operands, follow each other on one of them.
+  const int per = L.nm * L.vtiles, y = blockIdx.x >> 3;
+  const int unit = y / per * 8 + (blockIdx.x & 7), sub = y % per;
+  if (unit >= L.s.B * L.s.H * L.nseg) return;
+  const March& m = L.m[sub / L.vtiles];
+  const int v0 = sub % L.vtiles * VT;
+  if (v0 >= m.V) return;
+  const int h = unit % L.s.H, zb = unit / L.s.H, z = zb % L.nseg, b = zb / L.nseg;
+  const long long bh = (long long)b * L.s.H + h;
+  const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool rev = m.rev;
+  const int first = z * L.seg, last = min(first + L.seg, L.s.T), chunks = (last - first + C - 1) / C;
+  const int valid = valid_tokens(L.s, b);
+  const float l2 = decay_log2(L.s.log_decay, h);
+  auto power = [&](int n) { return n < 0 ? 0.f : exp2f(l2 * (float)n); };
+
+  const T* pa = static_cast<const T*>(m.a.p) + b * m.a.sb + (h / m.a.div) * m.a.sh;
+  const T* pb = static_cast<const T*>(m.b.p) + b * m.b.sb + (h / m.b.div) * m.b.sh;
+  const T* pc = static_cast<const T*>(m.c.p) + b * m.c.sb + (h / m.c.div) * m.c.sh + v0;
+
+  // the wavefront's tiles of P: (row tile, column tile), and their decays
+  int pi[NP], pj[NP];
+  float pd[NP][4];
+  if constexpr (OUT) {
+#pragma unroll
+    for (int n = 0; n < NP; n++) {
+      const int idx = w + 4 * n;
+      int r = 0;
+      while ((r + 1) * (r + 2) / 2 <= idx) r++;
+      const int c = idx - r * (r + 1) / 2;
+      pi[n] = rev ? c : r, pj[n] = rev ? r : c;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int d = 16 * pi[n] + i16 - (16 * pj[n] + 4 * g + e);
+        pd[n][e] = m.p * power(rev ? -d : d);
+      }
+    }
+    // tiles on the other side of the diagonal stay zero
+    for (int i = threadIdx.x; i < (int)sizeof(tp) / 16; i += 256) reinterpret_cast<uint4*>(&tp)[i] = make_uint4(0, 0, 0, 0);
+  }
+
+  // decays that depend on the tokens in a chunk: of the rows that see the entering state, of the state, and of
+  // the tokens that are added to it
+  float fi[MT], gn, wj[JS][8];
+  int have = -1;
+  auto decays = [&](int n) {
+    have = n;
+    gn = power(n);
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+      const int i = 16 * t + i16;
+      fi[t] = m.x * (rev ? power(n - 1 - i) : power(i + 1));
+    }
+#pragma unroll
+    for (int s = 0; s < JS; s++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int j = 32 * s + 4 * g + (e & 3) + 16 * (e >> 2);
+        wj[s][e] = j < n ? m.w * power(rev ? j + 1 : n - 1 - j) : 0.f;
+      }
+  };
+
+  f32x4 S[KT / 16][VW];
+  {
+    const float* s0 = m.s0 ? m.s0 + bh * m.s0_bh + z * m.s0_seg : nullptr;
+#pragma unroll
+    for (int a = 0; a < KT / 16; a++)
+#pragma unroll
+      for (int v = 0; v < VW; v++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int kk = 16 * a + 4 * g + r, vv = v0 + 16 * (w * VW + v) + i16;
+          S[a][v][r] = s0 && kk < m.K && vv < m.V ? s0[(long long)kk * m.sk + (long long)vv * m.sv] : 0.f;
+        }
+  }
+
+  Stage<T, C, KT> ga, gb;
+  Stage<T, C, VT> gc;
+  auto start = [&](int c) { return first + (rev ? chunks - 1 - c : c) * C; };
+  auto fetch = [&](int c) {
+    const int t0 = start(c), n = min(max(min(valid, last) - t0, 0), C);
+    if constexpr (OUT) ga.load(pa + t0 * m.a.st, m.a.st, n, m.K);
+    gb.load(pb + t0 * m.b.st, m.b.st, n, m.K);
+    gc.load(pc + t0 * m.c.st, m.c.st, n, m.V - v0);
+  };
+  fetch(0);
+
+  for (int c = 0; c < chunks; c++) {
+    const int t0 = start(c), n = min(max(min(valid, last) - t0, 0), C);
+    if (n != have) decays(n);
+    __syncthreads();
+    if constexpr (OUT) ga.store(ta);
+    gb.store(tb);
+    gc.store(tc);
+    if (c + 1 < chunks) fetch(c + 1);
+    __syncthreads();
+
+    f32x4 o[MT][VW];
+    if constexpr (OUT) {
+      // P^T tiles: rows j, columns i
+#pragma unroll
+      for (int t = 0; t < NP; t++) {
+        if (w + 4 * t < TILES) {
+          f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < KS; k++) product(tb.rows(16 * pj[t], 32 * k, i16, g), ta.rows(16 * pi[t], 32 * k, i16, g), d);
+          // stored in the order of the transposing reads' rows: 16 * (j / 16 % 2) + 4 g + e at 8 g + 4 (j / 16 % 2) + e
+          u16* q = &tp.v[0][16 * pi[t] + i16][32 * (pj[t] >> 1) + 8 * g + 4 * (pj[t] & 1)];
+          const float x0 = d[0] * pd[t][0], x1 = d[1] * pd[t][1], x2 = d[2] * pd[t][2], x3 = d[3] * pd[t][3];
+          if constexpr (NS == 1) {
+            *reinterpret_cast<uint2*>(q) = make_uint2(ops::pack_bf16(x0, x1), ops::pack_bf16(x2, x3));
+          } else {
+            uint2 hh, mm, ll;
+            split2(x0, x1, hh.x, mm.x, ll.x);
+            split2(x2, x3, hh.y, mm.y, ll.y);
+            *reinterpret_cast<uint2*>(q) = hh;
+            *reinterpret_cast<uint2*>(q + C * (C + 8)) = mm;
+            *reinterpret_cast<uint2*>(q + 2 * C * (C + 8)) = ll;
+          }
         }
       }
-      o *= m.x;
+      // a X, transposed: rows vv, columns i
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int v = 0; v < VW; v++) o[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        Frag<NS> fs[VW];
+#pragma unroll
+        for (int v = 0; v < VW; v++) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = S[2 * k + (e >> 2)][v][e & 3];
+          fs[v] = split8<NS>(x);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+          const Frag<NS> fa = ta.rows_acc(16 * t, 32 * k, i16, g);
+#pragma unroll
+          for (int v = 0; v < VW; v++) product(fs[v], fa, o[t][v]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int v = 0; v < VW; v++) o[t][v] *= fi[t];
+      __syncthreads();
     }
-    o += __shfl_xor(o, 16);
-    o += __shfl_xor(o, 32);
-    if (in && r == 0) {
-      const long long q = (((long long)b * s.T + t) * s.H + h) * m.V + col;
-      if (m.out_f32) static_cast<float*>(m.out)[q] = o;
-      else ops::put(static_cast<T*>(m.out) + q, o);
+
+    // c's channels as an operand, tokens along the sum
+    Frag<NS> fc[JS][VW];
+#pragma unroll
+    for (int s = 0; s < JS; s++)
+#pragma unroll
+      for (int v = 0; v < VW; v++) fc[s][v] = tc.cols(32 * s, 16 * (w * VW + v), i16, g);
+    if constexpr (OUT) {
+#pragma unroll
+      for (int s = 0; s < JS; s++)
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+          if (rev ? 2 * s + 1 >= t : 2 * s <= t) {
+            const Frag<NS> fp = tp.rows(16 * t, 32 * s, i16, g);
+#pragma unroll
+            for (int v = 0; v < VW; v++) product(fc[s][v], fp, o[t][v]);
+          }
+#pragma unroll
+      for (int t = 0; t < MT; t++) {
+        const int tok = t0 + 16 * t + i16;
+        if (tok < last) {
+#pragma unroll
+          for (int v = 0; v < VW; v++) {
+            const int vv = v0 + 16 * (w * VW + v) + 4 * g;
+            if (vv < m.V) {
+              const long long at = (((long long)b * L.s.T + tok) * L.s.H + h) * m.V + vv;
+              const float x[4] = {o[t][v][0], o[t][v][1], o[t][v][2], o[t][v][3]};
+              if (m.out_f32) ops::store(static_cast<float*>(m.out) + at, x);
+              else ops::store(static_cast<T*>(m.out) + at, x);
+            }
+          }
+        }
+      }
+    }
+
+    // the state: decayed, and the chunk's tokens added
+    Frag<3> fw[JS][VW];
+#pragma unroll
+    for (int s = 0; s < JS; s++)
+#pragma unroll
+      for (int v = 0; v < VW; v++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x[e] = 0.f;
+#pragma unroll
+          for (int p = NS - 1; p >= 0; p--) x[e] += (float)fc[s][v].p[p][e];
+          x[e] *= wj[s][e];
+        }
+        fw[s][v] = split8<3>(x);
+      }
+#pragma unroll
+    for (int a = 0; a < KT / 16; a++) {
+#pragma unroll
+      for (int v = 0; v < VW; v++) S[a][v] *= gn;
+#pragma unroll
+      for (int s = 0; s < JS; s++) {
+        const Frag<NS> fb = tb.cols(32 * s, 16 * a, i16, g);
+#pragma unroll
+        for (int v = 0; v < VW; v++) product(fb, fw[s][v], S[a][v]);
+      }
     }
   }
-  if (m.s1)
+
+  if (m.s1) {
+    float* s1 = m.s1 + bh * m.s1_bh + z * m.s1_seg;
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-      const int kk = r + 4 * i;
-      if (in && kk < m.K) m.s1[at + (long long)kk * m.sk] = m.rev && n ? x[i] * g : x[i];
-    }
+    for (int a = 0; a < KT / 16; a++)
+#pragma unroll
+      for (int v = 0; v < VW; v++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int kk = 16 * a + 4 * g + r, vv = v0 + 16 * (w * VW + v) + i16;
+          if (kk < m.K && vv < m.V) s1[(long long)kk * m.sk + (long long)vv * m.sv] = S[a][v][r];
+        }
+  }
+}
+
+// The states that enter the segments, from those that the segments make of nothing, in place; and the last one.
+// Lane: four elements. Sixteen segments are read ahead.
+struct Scan {
+  float* seg;  // [bh][nseg][n]
+  const float* s0;
+  float* s1;
+  int n, rev;
+};
+struct ScanLaunch {
+  Scan c[2];
+  Shape s;
+  int nseg, seg;
+};
+__global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
+  const Scan& c = L.c[blockIdx.y];
+  const int tiles = (c.n + 1023) / 1024, bh = blockIdx.x / tiles, e = ((blockIdx.x - bh * tiles) * 256 + threadIdx.x) * 4;
+  if (e >= c.n) return;
+  const int h = bh % L.s.H, b = bh / L.s.H, valid = valid_tokens(L.s, b);
+  const float l2 = decay_log2(L.s.log_decay, h);
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c.s0) ops::load(c.s0 + (long long)bh * c.n + e, x);
+  float* p = c.seg + (long long)bh * L.nseg * c.n + e;
+  constexpr int AHEAD = 16;
+  for (int z0 = 0; z0 < L.nseg; z0 += AHEAD) {
+    float u[AHEAD][4];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (z0 + i < L.nseg) ops::load(p + (long long)(c.rev ? L.nseg - 1 - z0 - i : z0 + i) * c.n, u[i]);
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+      if (z0 + i < L.nseg) {
+        const int z = c.rev ? L.nseg - 1 - z0 - i : z0 + i;
+        const float d = exp2f(l2 * (float)min(max(valid - z * L.seg, 0), L.seg));
+        ops::store(p + (long long)z * c.n, x);
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = x[k] * d + u[i][k];
+      }
+  }
+  if (c.s1) ops::store(c.s1 + (long long)bh * c.n + e, x);
 }
 
 // Sum over the query heads that share a key/value head: out [rows][Hk][D] from in [rows][H][D].
