@@ -2,15 +2,16 @@
 //   r = x + s . act(g) . (y ry) . wp,   h = (r rr) . wq,   rz = 1 / sqrt(mean z^2 + eps)
 // With gr, gh the gradients of r and h, r^ = r rr and y^ = y ry:
 //   dr = gr + rr (gh wq - r^ mean(gh wq r^)),      dx = dr,   dwq = sum gh r^
-//   ds = sum dr act(g) y^ wp,   dg = dr s y^ wp act'(g),   dn = dr s act(g),   dwp = sum dn y^
-//   dy = ry (dn wp - y^ mean(dn wp y^))
-// r is not read back, it is made again from x, y and g: its stored value is rounded, and the sums over
-// rows of the weights' gradients would be off by that rounding.
+//   dg = dr s y^ wp act'(g),   dn = dr s act(g),   dy = ry (dn wp - y^ mean(dn wp y^))
+//   ds = wp t,  dwp = s t  with  t = sum dr act(g) y^
+// The weights leave the sums over rows, so that ds and dwp are one sum; so does a gate that many rows
+// share, whose gradient is s wp act'(g) sum dr y^. r is not read back, it is made again from x, y and g: its
+// stored value is rounded, and the weights' gradients would be off by that rounding.
 //
-// A row lies in the registers of one wavefront, or of one workgroup where it is longer than 1024
-// channels: every array crosses memory once. A workgroup takes a run of rows, so that the weights are
-// read once for all of them and the sums over rows stay in registers until its end; the parts it leaves
-// are added by a second kernel, in a fixed order.
+// A row lies in the registers of one workgroup, 8 channels to a lane (16 beyond 8192 channels): every array crosses
+// memory once. A workgroup takes a run of rows and reads the next one before it works on this one (up to 4096 channels);
+// sums over rows stay in registers until its end, and the parts it leaves are added by a second kernel in a
+// fixed order. Bound by memory.
 #pragma once
 #include "opsio.hpp"
 
@@ -21,9 +22,9 @@ struct Args {
   const void *x, *y, *gate, *gr, *gh;
   long long sx, sy, sg, sgr, sgh;
   const float *wq, *wp, *sc;
-  void *r, *h;           // forward
-  void *dx, *dy, *dgate; // backward; dgate only where each row has its own gate
-  float* parts;          // [quantity][part][C]: dwq, dwp, ds, and the gate's where rows share one
+  void *r, *h;            // forward
+  void *dx, *dy, *dgate;  // backward; dgate only where each row has its own gate
+  float* parts;           // [quantity][part][C]: dwq, t, and the gate's where rows share one
   long long rows, gate_rows, block_rows;  // block_rows: rows that may share a workgroup
   int C, act, part_rows, parts_per_block;
   long long nparts;
@@ -45,231 +46,333 @@ __device__ __forceinline__ float activate(int act, float g, float* d) {
   return g * s;
 }
 
-// Sums of N values over the lanes of a row: W wavefronts.
-template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], int W, float* lds) {
-#pragma unroll
-  for (int i = 0; i < N; i++)
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v[i] += __shfl_xor(v[i], o);
-  if (W == 1) return;
-  const int w = threadIdx.x >> 6;
-  __syncthreads();  // the last sum has been read
-  if ((threadIdx.x & 63) == 0)
-#pragma unroll
-    for (int i = 0; i < N; i++) lds[w * N + i] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    v[i] = 0.f;
-    for (int j = 0; j < W; j++) v[i] += lds[j * N + i];
-  }
+// Sum over the 64 lanes: within 16 by DPP (xor 1, xor 2, and mirrors of 8 and 16), then the four rows.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane(float x, int l) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x += dpp<0xB1>(x);
+  x += dpp<0x4E>(x);
+  x += dpp<0x141>(x);
+  x += dpp<0x140>(x);
+  return (lane(x, 0) + lane(x, 16)) + (lane(x, 32) + lane(x, 48));
 }
 
-// The channels of a lane: vector e of VEC at (e * lanes + lane) * VEC.
-template <class T, int VEC, int NV>
-__device__ __forceinline__ void get(const T* p, int lane, int lanes, int C, float (&v)[NV * VEC], float fill) {
+// Sums over the workgroup's W wavefronts. Successive sums use the two buffers in turn, so that one barrier each is
+// enough: who writes a buffer again has passed the barrier that follows its last reading.
+struct Sums {
+  float v[2][2][16];
+};
+struct Reduce {
+  Sums& s;
+  int W, turn;
+  template <int N>
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
-  for (int e = 0; e < NV; e++) {
-    const int at = (e * lanes + lane) * VEC;
-    float t[VEC];
-    if (at < C) ops::load(p + at, t);
+    for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+    if (W == 1) return;
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0)
 #pragma unroll
-    for (int i = 0; i < VEC; i++) v[e * VEC + i] = at < C ? t[i] : fill;
+      for (int i = 0; i < N; i++) s.v[turn][i][w] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      v[i] = 0.f;
+      for (int j = 0; j < W; j++) v[i] += s.v[turn][i][j];
+    }
+    turn ^= 1;
   }
-}
-template <class T, int VEC, int NV>
-__device__ __forceinline__ void set(T* p, int lane, int lanes, int C, const float (&v)[NV * VEC]) {
+};
+
+// A lane's N channels of a row, as they are in memory (bf16 two to a register, unless they come one by
+// one): vector e of VEC at (e * lanes + lane) * VEC.
+template <class T, int VEC, int N>
+struct Row {
+  static constexpr int PER = VEC == 1 ? 1 : 4 / (int)sizeof(T), WORDS = VEC / PER;
+  uint32_t w[N / PER];
+  __device__ __forceinline__ void load(const void* base, long long row, long long stride, int C) {
+    const T* p = static_cast<const T*>(base) + row * stride;
 #pragma unroll
-  for (int e = 0; e < NV; e++) {
-    const int at = (e * lanes + lane) * VEC;
+    for (int e = 0; e < N / VEC; e++) {
+      const int at = (e * (int)blockDim.x + (int)threadIdx.x) * VEC;
+      uint32_t* d = w + e * WORDS;
+#pragma unroll
+      for (int i = 0; i < WORDS; i++) d[i] = 0;
+      if (at < C) {
+        if constexpr (WORDS == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p + at);
+          d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+        } else if constexpr (WORDS == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p + at);
+          d[0] = v.x, d[1] = v.y;
+        } else if constexpr (sizeof(T) == 4) {
+          d[0] = __float_as_uint(p[at]);
+        } else {
+          d[0] = (uint32_t)p[at] << 16;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (PER == 2) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return __uint_as_float(w[i]);
+  }
+};
+template <class T, int VEC, int N>
+__device__ __forceinline__ void put_row(void* base, long long row, int C, const float (&x)[N]) {
+  T* p = static_cast<T*>(base) + row * C;
+#pragma unroll
+  for (int e = 0; e < N / VEC; e++) {
+    const int at = (e * (int)blockDim.x + (int)threadIdx.x) * VEC;
     float t[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; i++) t[i] = v[e * VEC + i];
+    for (int i = 0; i < VEC; i++) t[i] = x[e * VEC + i];
     if (at < C) ops::store(p + at, t);
   }
 }
-
-template <class T, int VEC, int NV, int BLK, bool Y>
-__global__ __launch_bounds__(BLK) void fwd_kernel(Args A) {
-  constexpr int N = VEC * NV;
-  __shared__ float lds[16 * 2];
-  // rows of one wavefront: four to a workgroup; else one row to a workgroup
-  const int W = A.C <= 64 * N ? 1 : blockDim.x >> 6, lanes = 64 * W;
-  const int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x, group = W == 1 ? threadIdx.x >> 6 : 0;
-  const int groups = W == 1 ? blockDim.x >> 6 : 1;
-  const long long first = (long long)blockIdx.x * A.part_rows, last = min(first + A.part_rows, A.rows);
-  float wq[N], wp[N], sc[N];
-  get<float, VEC, NV>(A.wq, lane, lanes, A.C, wq, 0.f);
-  if constexpr (Y) {
+// weights, 1 where there are none
+template <int VEC, int N>
+__device__ __forceinline__ void weights(const float* p, int C, float (&x)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; i++) wp[i] = sc[i] = 1.f;
-    if (A.wp) get<float, VEC, NV>(A.wp, lane, lanes, A.C, wp, 0.f);
-    if (A.sc) get<float, VEC, NV>(A.sc, lane, lanes, A.C, sc, 0.f);
+  for (int e = 0; e < N / VEC; e++) {
+    const int at = (e * (int)blockDim.x + (int)threadIdx.x) * VEC;
+    float t[VEC];
+    if (p && at < C) ops::load(p + at, t);
+#pragma unroll
+    for (int i = 0; i < VEC; i++) x[e * VEC + i] = !p ? 1.f : at < C ? t[i] : 0.f;
+  }
+}
+
+template <class T, int VEC, int N, int BLK, bool Y>
+__global__ __launch_bounds__(BLK) void fwd_kernel(Args A) {
+  constexpr bool AHEAD = BLK <= 512;  // 1024 lanes leave each 128 registers: none for a row in advance
+  __shared__ Sums sums;
+  Reduce reduce = {sums, (int)blockDim.x >> 6, 0};
+  const long long first = (long long)blockIdx.x * A.part_rows, last = min(first + A.part_rows, A.rows);
+  float wq[N], ws[N];
+  weights<VEC>(A.wq, A.C, wq);
+  if constexpr (Y) {
+    float sc[N];
+    weights<VEC>(A.wp, A.C, ws);
+    weights<VEC>(A.sc, A.C, sc);
+#pragma unroll
+    for (int i = 0; i < N; i++) ws[i] *= sc[i];
   }
   const float inv = 1.f / (float)A.C;
-  for (long long row = first + group; row < last; row += groups) {
-    float x[N], s[1];
-    get<T, VEC, NV>(static_cast<const T*>(A.x) + row * A.sx, lane, lanes, A.C, x, 0.f);
+  Row<T, VEC, N> nx, ny, ng;
+  auto fetch = [&](long long row) {
+    nx.load(A.x, row, A.sx, A.C);
     if constexpr (Y) {
-      float y[N], g[N], d;
-      get<T, VEC, NV>(static_cast<const T*>(A.y) + row * A.sy, lane, lanes, A.C, y, 0.f);
-      if (A.gate) get<T, VEC, NV>(static_cast<const T*>(A.gate) + row / A.gate_rows * A.sg, lane, lanes, A.C, g, 0.f);
-      float ry = 1.f;
+      ny.load(A.y, row, A.sy, A.C);
+      if (A.gate) ng.load(A.gate, A.gate_rows == 1 ? row : row / A.gate_rows, A.sg, A.C);
+    }
+  };
+  if (AHEAD) fetch(first);
+  for (long long row = first; row < last; row++) {
+    if (!AHEAD) fetch(row);
+    const Row<T, VEC, N> rx = nx, ry = ny, rg = ng;
+    if (AHEAD && row + 1 < last) fetch(row + 1);
+    float x[N], s[1];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = rx[i];
+    if constexpr (Y) {
+      float f = 1.f, d;
       if (A.wp) {
         s[0] = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; i++) s[0] += y[i] * y[i];
-        row_sum(s, W, lds);
-        ry = 1.f / sqrtf(s[0] * inv + A.eps);
+        for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
+        reduce(s);
+        f = 1.f / sqrtf(s[0] * inv + A.eps);
       }
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        float m = y[i] * ry * wp[i] * sc[i];
-        if (A.gate) m *= activate(A.act, g[i], &d);
+        float m = ry[i] * f * ws[i];
+        if (A.gate) m *= activate(A.act, rg[i], &d);
         x[i] += m;
       }
-      set<T, VEC, NV>(static_cast<T*>(A.r) + row * A.C, lane, lanes, A.C, x);
+      put_row<T, VEC>(A.r, row, A.C, x);
     }
     s[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < N; i++) s[0] += x[i] * x[i];
-    row_sum(s, W, lds);
-    const float rr = 1.f / sqrtf(s[0] * inv + A.eps);
+    reduce(s);
+    const float f = 1.f / sqrtf(s[0] * inv + A.eps);
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] *= rr * wq[i];
-    set<T, VEC, NV>(static_cast<T*>(A.h) + row * A.C, lane, lanes, A.C, x);
+    for (int i = 0; i < N; i++) x[i] *= f * wq[i];
+    put_row<T, VEC>(A.h, row, A.C, x);
   }
 }
 
-// Adds the four wavefronts' values of one quantity and writes the workgroup's part.
-template <int VEC, int NV>
-__device__ __forceinline__ void put_part(float* part, float* lds, int lane, int lanes, int C, int group, int groups,
-                                         float (&v)[NV * VEC]) {
-  if (groups > 1) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NV * VEC; i++) lds[(group * NV * VEC + i) * 64 + lane] = v[i];
-    __syncthreads();
-    if (group) return;
-    for (int g = 1; g < groups; g++)
-#pragma unroll
-      for (int i = 0; i < NV * VEC; i++) v[i] += lds[(g * NV * VEC + i) * 64 + lane];
-  }
-  set<float, VEC, NV>(part, lane, lanes, C, v);
-}
-
-template <class T, int VEC, int NV, int BLK, bool Y>
+template <class T, int VEC, int N, int BLK, bool Y>
 __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
-  constexpr int N = VEC * NV;
-  __shared__ float lds[4 * N * 64];
-  const int W = A.C <= 64 * N ? 1 : blockDim.x >> 6, lanes = 64 * W;
-  const int lane = W == 1 ? threadIdx.x & 63 : threadIdx.x, group = W == 1 ? threadIdx.x >> 6 : 0;
-  const int groups = W == 1 ? blockDim.x >> 6 : 1;
+  constexpr bool AHEAD = BLK <= 512;  // 1024 lanes leave each 128 registers: none for a row in advance
+  __shared__ Sums sums;
+  Reduce reduce = {sums, (int)blockDim.x >> 6, 0};
   const long long part = blockIdx.x, block = part / A.parts_per_block;
   const long long first = block * A.block_rows + (part - block * A.parts_per_block) * A.part_rows;
   const long long last = min(min(first + A.part_rows, (block + 1) * A.block_rows), A.rows);
-  float wq[N], wp[N], sc[N], dwq[N], dwp[N], dsc[N], dgs[N];
-  get<float, VEC, NV>(A.wq, lane, lanes, A.C, wq, 0.f);
-#pragma unroll
-  for (int i = 0; i < N; i++) wp[i] = sc[i] = 1.f, dwq[i] = dwp[i] = dsc[i] = dgs[i] = 0.f;
-  if constexpr (Y) {
-    if (A.wp) get<float, VEC, NV>(A.wp, lane, lanes, A.C, wp, 0.f);
-    if (A.sc) get<float, VEC, NV>(A.sc, lane, lanes, A.C, sc, 0.f);
-  }
+  const bool shared = A.gate && A.gate_rows > 1;
   const float inv = 1.f / (float)A.C;
-  const bool shared_gate = A.gate_rows > 1;
-  for (long long row = first + group; row < last; row += groups) {
-    float r[N], y[N], g[N], gr[N], gh[N];
-    get<T, VEC, NV>(static_cast<const T*>(A.x) + row * A.sx, lane, lanes, A.C, r, 0.f);
-    if constexpr (Y) {
-      get<T, VEC, NV>(static_cast<const T*>(A.y) + row * A.sy, lane, lanes, A.C, y, 0.f);
-      if (A.gate) get<T, VEC, NV>(static_cast<const T*>(A.gate) + row / A.gate_rows * A.sg, lane, lanes, A.C, g, 0.f);
-    }
+  float wq[N], wp[N], sc[N], dwq[N], t[N];
+  weights<VEC>(A.wq, A.C, wq);
 #pragma unroll
-    for (int i = 0; i < N; i++) gr[i] = gh[i] = 0.f;
-    if (A.gr) get<T, VEC, NV>(static_cast<const T*>(A.gr) + row * A.sgr, lane, lanes, A.C, gr, 0.f);
-    if (A.gh) get<T, VEC, NV>(static_cast<const T*>(A.gh) + row * A.sgh, lane, lanes, A.C, gh, 0.f);
-    float ry = 1.f, s[1], act[N], dact[N];
+  for (int i = 0; i < N; i++) dwq[i] = t[i] = 0.f;
+  if constexpr (Y) {
+    weights<VEC>(A.wp, A.C, wp);
+    weights<VEC>(A.sc, A.C, sc);
+  }
+  Row<T, VEC, N> nx, ny, ng, nr, nh;
+  auto fetch = [&](long long row) {
+    nx.load(A.x, row, A.sx, A.C);
+    if constexpr (Y) {
+      ny.load(A.y, row, A.sy, A.C);
+      if (A.gate) ng.load(A.gate, shared ? row / A.gate_rows : row, A.sg, A.C);
+    }
+    if (A.gr) nr.load(A.gr, row, A.sgr, A.C);
+    if (A.gh) nh.load(A.gh, row, A.sgh, A.C);
+  };
+  if (!A.gr) nr = {};
+  if (!A.gh) nh = {};
+  if (AHEAD) fetch(first);
+  Row<T, VEC, N> rg = {};
+  for (long long row = first; row < last; row++) {
+    if (!AHEAD) fetch(row);
+    const Row<T, VEC, N> rx = nx, ry = ny, rr = nr, rh = nh;
+    rg = ng;
+    if (AHEAD && row + 1 < last) fetch(row + 1);
+    float r[N], y[N], act[N], s[1], fy = 1.f, d;
+#pragma unroll
+    for (int i = 0; i < N; i++) r[i] = rx[i];
     if constexpr (Y) {
       if (A.wp) {
         s[0] = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; i++) s[0] += y[i] * y[i];
-        row_sum(s, W, lds);
-        ry = 1.f / sqrtf(s[0] * inv + A.eps);
+        for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
+        reduce(s);
+        fy = 1.f / sqrtf(s[0] * inv + A.eps);
       }
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        act[i] = dact[i] = 1.f;
-        if (A.gate) act[i] = activate(A.act, g[i], &dact[i]);
-        y[i] *= ry;
+        act[i] = A.gate ? activate(A.act, rg[i], &d) : 1.f;
+        y[i] = ry[i] * fy;
         r[i] += y[i] * wp[i] * sc[i] * act[i];
       }
     }
-    float t[2] = {0.f, 0.f};
+    float q[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; i++) t[0] += r[i] * r[i], t[1] += gh[i] * wq[i] * r[i];
-    row_sum(t, W, lds);
-    const float rr = 1.f / sqrtf(t[0] * inv + A.eps), mean = t[1] * rr * inv;
+    for (int i = 0; i < N; i++) q[0] += r[i] * r[i], q[1] += rh[i] * wq[i] * r[i];
+    reduce(q);
+    const float fr = 1.f / sqrtf(q[0] * inv + A.eps), mean = q[1] * fr * inv;
+    float dr[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      r[i] *= rr;
-      dwq[i] += gh[i] * r[i];
-      gr[i] += rr * (gh[i] * wq[i] - r[i] * mean);
+      r[i] *= fr;
+      dwq[i] += rh[i] * r[i];
+      dr[i] = rr[i] + fr * (rh[i] * wq[i] - r[i] * mean);
     }
-    set<T, VEC, NV>(static_cast<T*>(A.dx) + row * A.C, lane, lanes, A.C, gr);
+    put_row<T, VEC>(A.dx, row, A.C, dr);
     if constexpr (Y) {
+      if (shared) {
 #pragma unroll
-      for (int i = 0; i < N; i++) {
-        const float n = y[i] * wp[i];
-        dsc[i] += gr[i] * act[i] * n;
-        g[i] = gr[i] * sc[i] * n * dact[i];
-        dgs[i] += g[i];
-        gr[i] *= sc[i] * act[i];
+        for (int i = 0; i < N; i++) t[i] += dr[i] * y[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) t[i] += dr[i] * y[i] * act[i];
       }
-      if (A.gate && !shared_gate) set<T, VEC, NV>(static_cast<T*>(A.dgate) + row * A.C, lane, lanes, A.C, g);
+      if (A.gate && !shared) {
+        float g[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          activate(A.act, rg[i], &d);
+          g[i] = dr[i] * sc[i] * y[i] * wp[i] * d;
+        }
+        put_row<T, VEC>(A.dgate, row, A.C, g);
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) dr[i] *= sc[i] * act[i];
       if (A.wp) {
         s[0] = 0.f;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-          dwp[i] += gr[i] * y[i];
-          gr[i] *= wp[i];
-          s[0] += gr[i] * y[i];
+          dr[i] *= wp[i];
+          s[0] += dr[i] * y[i];
         }
-        row_sum(s, W, lds);
+        reduce(s);
         const float my = s[0] * inv;
 #pragma unroll
-        for (int i = 0; i < N; i++) gr[i] = ry * (gr[i] - y[i] * my);
+        for (int i = 0; i < N; i++) dr[i] = fy * (dr[i] - y[i] * my);
       }
-      set<T, VEC, NV>(static_cast<T*>(A.dy) + row * A.C, lane, lanes, A.C, gr);
+      put_row<T, VEC>(A.dy, row, A.C, dr);
     }
   }
-  const long long q = A.nparts * A.C;
-  float* out = A.parts + part * A.C;
-  put_part<VEC, NV>(out, lds, lane, lanes, A.C, group, groups, dwq);
+  put_row<float, VEC>(A.parts, part, A.C, dwq);
   if constexpr (Y) {
-    if (A.wp) put_part<VEC, NV>(out + q, lds, lane, lanes, A.C, group, groups, dwp);
-    if (A.sc) put_part<VEC, NV>(out + 2 * q, lds, lane, lanes, A.C, group, groups, dsc);
-    if (A.gate && shared_gate) put_part<VEC, NV>(out + 3 * q, lds, lane, lanes, A.C, group, groups, dgs);
+    if (shared) {
+      float g[N], d;
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float a = activate(A.act, rg[i], &d);
+        g[i] = t[i] * sc[i] * wp[i] * d;
+        t[i] *= a;
+      }
+      put_row<float, VEC>(A.parts, 2 * A.nparts + part, A.C, g);
+    }
+    put_row<float, VEC>(A.parts, A.nparts + part, A.C, t);
   }
 }
 
-// out[block][c] = sum of `per` consecutive parts
-template <class T>
-__global__ __launch_bounds__(256) void sum_kernel(const float* parts, T* out, int C, int per) {
-  __shared__ float lds[4][64];
-  const int tiles = (C + 63) / 64, block = blockIdx.x / tiles;
-  const int c = (blockIdx.x - block * tiles) * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
-  const float* p = parts + (long long)block * per * C + c;
+// The sums of the parts. Workgroups take 32 columns of one quantity: the nparts parts of dwq and of t, which gives
+// dwp and ds, then for each gate that rows share its `per` consecutive parts.
+struct SumArgs {
+  const float *parts, *wp, *sc;
+  float *dwq, *dwp, *ds;
+  void* dgate;
+  int C, bf16, y;
+  long long nparts, per;
+};
+__global__ __launch_bounds__(1024) void sum_kernel(SumArgs A) {
+  __shared__ float lds[32][33];
+  const int tiles = (A.C + 31) / 32, which = blockIdx.x / tiles, lc = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int c = (blockIdx.x - which * tiles) * 32 + lc;
+  // which: 0 = dwq, 1 = t (where there is a y), then the gates
+  const int gate = which - (A.y ? 2 : 1);
+  const long long n = gate < 0 ? A.nparts : A.per, at = gate < 0 ? which * A.nparts : 2 * A.nparts + gate * A.per;
+  const float* p = A.parts + at * A.C + c;
   float s = 0.f;
-  if (c < C)
-    for (int i = g; i < per; i += 4) s += p[(long long)i * C];
-  lds[g][threadIdx.x & 63] = s;
+  if (c < A.C) {
+    long long i = g;
+    for (; i + 7 * 32 < n; i += 8 * 32) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = p[(i + 32 * k) * A.C];
+#pragma unroll
+      for (int k = 0; k < 8; k++) s += v[k];
+    }
+    for (; i < n; i += 32) s += p[i * A.C];
+  }
+  lds[g][lc] = s;
   __syncthreads();
-  if (g == 0 && c < C)
-    ops::put(out + (long long)block * C + c,
-             lds[0][threadIdx.x] + lds[1][threadIdx.x] + lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+  // 32 lanes add 32 rows: lane (g, lc) of the first wavefronts takes column g
+  s = lds[lc][g];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor(s, o);
+  const int col = (blockIdx.x - which * tiles) * 32 + g;
+  if (lc || col >= A.C) return;
+  if (which == 0) {
+    A.dwq[col] = s;
+  } else if (gate < 0) {
+    if (A.dwp) A.dwp[col] = A.sc ? A.sc[col] * s : s;
+    if (A.ds) A.ds[col] = A.wp ? A.wp[col] * s : s;
+  } else if (A.bf16) {
+    ops::put(static_cast<uint16_t*>(A.dgate) + (long long)gate * A.C + col, s);
+  } else {
+    static_cast<float*>(A.dgate)[(long long)gate * A.C + col] = s;
+  }
 }
 
 }  // namespace bn

@@ -44,71 +44,61 @@ hipError_t rotary(rot::Args a, long long tokens, bool interleaved, bool wide, hi
 
 // ---- norms ----
 
-// How a row lies in registers: VEC channels to a load, NV loads to a lane, `lanes` lanes to a row; the
-// fewest lanes that hold it in 16 channels each. Four rows to a workgroup where one wavefront holds a row.
+// How a row lies in registers: N channels to a lane, in loads of `vec`; the fewest wavefronts that hold it.
 struct RowShape {
-  int vec, nv, lanes, block;
+  int vec, n, waves;
 };
-RowShape row_shape(int C, bool wide) {
-  RowShape s;
-  s.vec = wide ? 4 : 1;
-  s.lanes = 64;
-  while (s.lanes * 16 < C) s.lanes *= 2;
-  const int per = (C + s.lanes - 1) / s.lanes;  // channels of a lane
-  s.nv = (per + 3) / 4;                         // in fours, whatever the loads
-  s.block = s.lanes == 64 ? 256 : s.lanes;
-  return s;
+RowShape row_shape(int C, int vec) {
+  const int n = C > 8192 ? 16 : 8;
+  return {vec, n, (C + 64 * n - 1) / (64 * n)};
 }
 
-// Rows in parts that one workgroup each takes: about 8 wavefronts for each of 256 CUs, no part across
-// rows of different gates.
+// Rows in parts that one workgroup each takes: about `fill` wavefronts for each of 256 CUs, no part across rows
+// of different gates.
 struct Parts {
   long long block_rows, blocks, nparts;
   int part_rows, per_block;
 };
-Parts parts_of(const sffft_blocknorm* p, const RowShape& s, bool shared_gate) {
+Parts parts_of(const sffft_blocknorm* p, const RowShape& s, bool shared_gate, int fill) {
   Parts q;
   q.block_rows = shared_gate ? p->gate_rows : p->rows;
   q.blocks = p->rows / q.block_rows;
-  const int at_once = s.lanes == 64 ? 4 : 1;
-  const long long want = std::max<long long>(1, 256 * 8 * 64 / s.block / q.blocks);
-  const long long rounds = (q.block_rows + at_once - 1) / at_once;
-  long long per = std::min(want, rounds);
-  q.part_rows = (int)std::min<long long>((rounds + per - 1) / per * at_once, INT_MAX / 2);
+  const long long want = std::max<long long>(1, 256 * fill / s.waves / q.blocks);
+  const long long per = std::min(want, q.block_rows);
+  q.part_rows = (int)std::min<long long>((q.block_rows + per - 1) / per, INT_MAX / 2);
   q.per_block = (int)((q.block_rows + q.part_rows - 1) / q.part_rows);
   q.nparts = q.blocks * q.per_block;
   return q;
 }
+// Registers allow about 12 wavefronts for the backward kernel and 24 for the forward one.
+constexpr int FILL_FWD = 24, FILL_BWD = 12;
 
-template <class T, int VEC, int NV, int BLK>
-void norm_launch(const bn::Args& a, bool y, bool backward, dim3 grid, dim3 block, hipStream_t st) {
+template <class T, int VEC, int N, int BLK>
+void norm_launch(const bn::Args& a, int waves, bool y, bool backward, dim3 grid, hipStream_t st) {
+  const dim3 block(64u * waves);
   if (backward) {
-    if (y) hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, NV, BLK, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, NV, BLK, false>), grid, block, 0, st, a);
+    if (y) hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, N, BLK, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, N, BLK, false>), grid, block, 0, st, a);
   } else {
-    if (y) hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, NV, BLK, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, NV, BLK, false>), grid, block, 0, st, a);
+    if (y) hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, N, BLK, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, N, BLK, false>), grid, block, 0, st, a);
   }
 }
-template <class T, int VEC, int BLK>
-void norm_nv(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
-  constexpr int Q = 4 / VEC;
-  const dim3 block((unsigned)s.block);
-  switch (s.nv) {
-    case 1: return norm_launch<T, VEC, Q, BLK>(a, y, backward, grid, block, st);
-    case 2: return norm_launch<T, VEC, 2 * Q, BLK>(a, y, backward, grid, block, st);
-    case 3: return norm_launch<T, VEC, 3 * Q, BLK>(a, y, backward, grid, block, st);
-    default: return norm_launch<T, VEC, 4 * Q, BLK>(a, y, backward, grid, block, st);
-  }
+template <class T, int VEC>
+void norm_vec(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
+  if (s.n == 16) norm_launch<T, VEC, 16, 1024>(a, s.waves, y, backward, grid, st);
+  else if (s.waves > 8) norm_launch<T, VEC, 8, 1024>(a, s.waves, y, backward, grid, st);
+  else if (s.waves > 4) norm_launch<T, VEC, 8, 512>(a, s.waves, y, backward, grid, st);
+  else norm_launch<T, VEC, 8, 256>(a, s.waves, y, backward, grid, st);
 }
 template <class T>
 hipError_t norm(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
-  if (s.vec == 4) {
-    if (s.block <= 256) norm_nv<T, 4, 256>(a, s, y, backward, grid, st);
-    else norm_nv<T, 4, 1024>(a, s, y, backward, grid, st);
+  if (s.vec == 8) {
+    if constexpr (sizeof(T) == 2) norm_vec<T, 8>(a, s, y, backward, grid, st);
+  } else if (s.vec == 4) {
+    norm_vec<T, 4>(a, s, y, backward, grid, st);
   } else {
-    if (s.block <= 256) norm_nv<T, 1, 256>(a, s, y, backward, grid, st);
-    else norm_nv<T, 1, 1024>(a, s, y, backward, grid, st);
+    norm_vec<T, 1>(a, s, y, backward, grid, st);
   }
   return hipGetLastError();
 }
@@ -143,15 +133,17 @@ bool apart(const Span* in, int ni, const Span* out, int no) {
   return true;
 }
 
-// Vector loads of four channels: every array's rows aligned to them.
-bool wide_rows(const sffft_blocknorm* p, const Span* all, int n, const long long* strides, int ns) {
+// The widest loads, of 16 bytes or of four channels, that every array's rows are aligned to; else one by one.
+int vector_of(const sffft_blocknorm* p, const Span* all, int n, const long long* strides, int ns, const float* const w[3]) {
   const int elem = p->io ? 2 : 4;
-  if (p->C % 4) return false;
-  for (int i = 0; i < n; i++)
-    if (!ops::aligned(all[i].p, 4 * elem)) return false;
-  for (int i = 0; i < ns; i++)
-    if (strides[i] % 4) return false;
-  return true;
+  for (int vec : {16 / elem, 4}) {
+    bool ok = p->C % vec == 0;
+    for (int i = 0; i < n; i++) ok = ok && ops::aligned(all[i].p, vec * elem);
+    for (int i = 0; i < ns; i++) ok = ok && strides[i] % vec == 0;
+    for (int i = 0; i < 3; i++) ok = ok && ops::aligned(w[i], 16);
+    if (ok) return vec;
+  }
+  return 1;
 }
 
 }  // namespace
@@ -239,10 +231,9 @@ int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, 
   if (!ops::aligned(r, elem) || !ops::aligned(h, elem) || !apart(in, 6, out, 2)) return SFFFT_EINVAL;
   const long long strides[] = {p->x, y ? p->y : 0, gate ? p->gate : 0};
   const Span act[] = {{x, 0}, {y, 0}, {gate, 0}, {r, 0}, {h, 0}};
-  bool wide = wide_rows(p, act, 5, strides, 3);
-  for (const float* w : {w_pre, w_post, scale}) wide = wide && ops::aligned(w, 16);
-  const RowShape s = row_shape(p->C, wide);
-  const Parts q = parts_of(p, s, false);
+  const float* const w[] = {w_pre, w_post, scale};
+  const RowShape s = row_shape(p->C, vector_of(p, act, 5, strides, 3, w));
+  const Parts q = parts_of(p, s, false, FILL_FWD);
   if (q.nparts > INT_MAX) return SFFFT_EINVAL;
   bn::Args a = {};
   a.x = x, a.y = y, a.gate = gate, a.sx = p->x, a.sy = p->y, a.sg = p->gate;
@@ -253,12 +244,11 @@ int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, 
                          "block norm launch");
 }
 
-// The parts of the forms with and without wide loads differ in nothing: row_shape's lanes do not depend on it.
 size_t sffft_blocknorm_work_bytes(const sffft_blocknorm* p, int has_y, int has_gate) {
   if (!valid_norm(p)) return 0;
   const bool shared = has_gate && p->gate_rows > 1;
-  const Parts q = parts_of(p, row_shape(p->C, true), shared);
-  return (size_t)(has_y ? shared ? 4 : 3 : 1) * q.nparts * p->C * 4;
+  const Parts q = parts_of(p, row_shape(p->C, 1), shared, FILL_BWD);  // the width of the loads changes nothing in it
+  return (size_t)(has_y ? shared ? 3 : 2 : 1) * q.nparts * p->C * 4;
 }
 
 int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, const void* gate, const float* w_pre,
@@ -287,10 +277,9 @@ int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, 
   if (!apart(in, 8, out, 7)) return SFFFT_EINVAL;
   const long long strides[] = {p->x, y ? p->y : 0, gate ? p->gate : 0, gr ? p->gr : 0, gh ? p->gh : 0};
   const Span act[] = {{x, 0}, {y, 0}, {gate, 0}, {gr, 0}, {gh, 0}, {dx, 0}, {dy, 0}, {dgate, 0}};
-  bool wide = wide_rows(p, act, 8, strides, 5);
-  for (const float* w : {w_pre, w_post, scale}) wide = wide && ops::aligned(w, 16);
-  const RowShape s = row_shape(p->C, wide);
-  const Parts q = parts_of(p, s, shared);
+  const float* const w[] = {w_pre, w_post, scale};
+  const RowShape s = row_shape(p->C, vector_of(p, act, 8, strides, 5, w));
+  const Parts q = parts_of(p, s, shared, FILL_BWD);
   if (q.nparts > INT_MAX) return SFFFT_EINVAL;
   bn::Args a = {};
   a.x = x, a.y = y, a.gate = gate, a.gr = gr, a.gh = gh;
@@ -302,23 +291,11 @@ int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, 
   hipStream_t st = (hipStream_t)stream;
   const auto run = p->io ? norm<uint16_t> : norm<float>;
   hipError_t err = run(a, s, y != nullptr, true, dim3((unsigned)q.nparts), st);
-  const unsigned tiles = (unsigned)((p->C + 63) / 64);
-  float* const sums[] = {dw_pre, dw_post, dscale};
-  for (int i = 0; i < 3 && err == hipSuccess; i++)
-    if (sums[i]) {
-      hipLaunchKernelGGL(bn::sum_kernel<float>, dim3(tiles), dim3(256), 0, st, a.parts + (size_t)i * q.nparts * p->C,
-                         sums[i], p->C, (int)q.nparts);
-      err = hipGetLastError();
-    }
-  if (err == hipSuccess && shared) {
-    const float* parts = a.parts + (size_t)3 * q.nparts * p->C;
-    const dim3 grid((unsigned)(tiles * q.blocks));
-    if (p->io)
-      hipLaunchKernelGGL(bn::sum_kernel<uint16_t>, grid, dim3(256), 0, st, parts, static_cast<uint16_t*>(dgate), p->C,
-                         q.per_block);
-    else
-      hipLaunchKernelGGL(bn::sum_kernel<float>, grid, dim3(256), 0, st, parts, static_cast<float*>(dgate), p->C,
-                         q.per_block);
+  if (err == hipSuccess) {
+    const bn::SumArgs u = {a.parts, w_post, scale, dw_pre, dw_post, dscale, shared ? dgate : nullptr, p->C, p->io,
+                           y != nullptr, q.nparts, q.per_block};
+    const long long sums = (y ? 2 : 1) + (shared ? q.blocks : 0);
+    hipLaunchKernelGGL(bn::sum_kernel, dim3((unsigned)((p->C + 31) / 32 * sums)), dim3(1024), 0, st, u);
     err = hipGetLastError();
   }
   return ops::hip_status(err, "block norm gradient launch");
