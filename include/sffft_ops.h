@@ -37,7 +37,8 @@ typedef struct sffft_linattn {
   int B, T, H, Hk;        /* H a multiple of Hk */
   int Dk, Dv;             /* multiples of 8, at most 128 */
   float scale;
-  long long q[3], k[3], v[3]; /* element strides (batch, token, head): multiples of 16 bytes */
+  long long q[3], k[3], v[3]; /* element strides (batch, token, head): multiples of 16 bytes, the token's
+                               * at most 2^24 - 128 */
   long long go[3];        /* of o's gradient (backward only) */
 } sffft_linattn;
 

@@ -13,6 +13,8 @@ using la::Operand;
 using la::Shape;
 
 constexpr int MAX_D = 128;
+// the rows of a chunk are addressed by 31-bit byte offsets: 64 of them in 2 bytes, 32 in 4
+constexpr long long MAX_TOKEN_STRIDE = (1 << 24) - MAX_D;
 
 bool valid_shape(const sffft_linattn* p) {
   if (!p || !ops::valid_io(p->io) || p->B < 1 || p->T < 1 || p->H < 1 || p->Hk < 1 || p->H % p->Hk) return false;
@@ -26,6 +28,7 @@ bool valid_input(const void* x, const long long s[3], const sffft_linattn* p, in
   if (!x || !ops::aligned(x, 16)) return false;
   for (int i = 0; i < 3; i++)
     if (s[i] * elem % 16) return false;
+  if (s[1] > MAX_TOKEN_STRIDE) return false;
   *bytes = ops::extent(s, p->B, p->T, heads, D, elem);
   return *bytes != 0;
 }

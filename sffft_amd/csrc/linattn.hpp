@@ -28,6 +28,7 @@ namespace la {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16;
 
 // One operand: element strides of (batch, token, head); head h of the march reads head h / div.
@@ -164,30 +165,32 @@ struct Tile {
 };
 
 // A chunk's rows of one operand on their way from memory to LDS: 16 bytes a piece, rows from n on and channels
-// from D on are zero and not read.
+// from D on are zero and not read: their lanes' offsets lie beyond the buffer's records. One lane offset serves
+// every piece, the rest is in scalar registers.
 template <class T, int C, int DT>
 struct Stage {
-  static constexpr int E = 16 / sizeof(T), PER = DT / E, N = C * PER / 256;
-  uint4 v[N];
+  static constexpr int E = 16 / sizeof(T), PER = DT / E, N = C * PER / 256, ROWS = 256 / PER;
+  static constexpr uint32_t RECORDS = 0x7fffffffu, OUTSIDE = 0x80000000u;
+  i32x4 v[N];
   __device__ __forceinline__ void load(const T* p, long long st, int n, int D) {
+    const int row = threadIdx.x / PER, col = threadIdx.x % PER * E;
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, RECORDS, 0x00027000);
+    const uint32_t at = col < D ? (uint32_t)(row * (int)st + col) * sizeof(T) : OUTSIDE;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int piece = threadIdx.x + 256 * i, row = piece / PER, col = piece % PER * E;
-      v[i] = make_uint4(0, 0, 0, 0);
-      if (row < n && col < D) v[i] = *reinterpret_cast<const uint4*>(p + row * st + col);
-    }
+    for (int i = 0; i < N; i++)
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, row + i * ROWS < n ? at : OUTSIDE, i * ROWS * (int)st * (int)sizeof(T), 0);
   }
   template <int NS, int L>
   __device__ __forceinline__ void store(Tile<NS, C, L>& t) const {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int piece = threadIdx.x + 256 * i, row = piece / PER, col = piece % PER * E;
+      const int row = threadIdx.x / PER + i * ROWS, col = threadIdx.x % PER * E;
       if constexpr (NS == 1) {
-        *reinterpret_cast<uint4*>(&t.v[0][row][col]) = v[i];
+        *reinterpret_cast<i32x4*>(&t.v[0][row][col]) = v[i];
       } else {
         uint2 h, m, l;
-        split2(__uint_as_float(v[i].x), __uint_as_float(v[i].y), h.x, m.x, l.x);
-        split2(__uint_as_float(v[i].z), __uint_as_float(v[i].w), h.y, m.y, l.y);
+        split2(__int_as_float(v[i].x), __int_as_float(v[i].y), h.x, m.x, l.x);
+        split2(__int_as_float(v[i].z), __int_as_float(v[i].w), h.y, m.y, l.y);
         *reinterpret_cast<uint2*>(&t.v[0][row][col]) = h;
         *reinterpret_cast<uint2*>(&t.v[1][row][col]) = m;
         *reinterpret_cast<uint2*>(&t.v[2][row][col]) = l;
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
       int r = 0;
       while ((r + 1) * (r + 2) / 2 <= idx) r++;
       const int c = idx - r * (r + 1) / 2;
-      pi[n] = rev ? c : r, pj[n] = rev ? r : c;
+      pi[n] = __builtin_amdgcn_readfirstlane(rev ? c : r), pj[n] = __builtin_amdgcn_readfirstlane(rev ? r : c);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int d = 16 * pi[n] + i16 - (16 * pj[n] + 4 * g + e);
@@ -398,9 +401,13 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
     }
 
     // the state: decayed, and the chunk's tokens added
-    Frag<3> fw[JS][VW];
 #pragma unroll
-    for (int s = 0; s < JS; s++)
+    for (int a = 0; a < KT / 16; a++)
+#pragma unroll
+      for (int v = 0; v < VW; v++) S[a][v] *= gn;
+#pragma unroll
+    for (int s = 0; s < JS; s++) {
+      Frag<3> fw[VW];
 #pragma unroll
       for (int v = 0; v < VW; v++) {
         float x[8];
@@ -411,17 +418,13 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
           for (int p = NS - 1; p >= 0; p--) x[e] += (float)fc[s][v].p[p][e];
           x[e] *= wj[s][e];
         }
-        fw[s][v] = split8<3>(x);
+        fw[v] = split8<3>(x);
       }
 #pragma unroll
-    for (int a = 0; a < KT / 16; a++) {
-#pragma unroll
-      for (int v = 0; v < VW; v++) S[a][v] *= gn;
-#pragma unroll
-      for (int s = 0; s < JS; s++) {
+      for (int a = 0; a < KT / 16; a++) {
         const Frag<NS> fb = tb.cols(32 * s, 16 * a, i16, g);
 #pragma unroll
-        for (int v = 0; v < VW; v++) product(fb, fw[s][v], S[a][v]);
+        for (int v = 0; v < VW; v++) product(fb, fw[v], S[a][v]);
       }
     }
   }

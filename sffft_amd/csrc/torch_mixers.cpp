@@ -73,6 +73,7 @@ Tensor rows16(const Tensor& t) {
   const int64_t e = t.element_size();
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
   for (int64_t d = 0; d + 1 < t.dim(); d++) ok = ok && t.stride(d) >= 0 && t.stride(d) * e % 16 == 0;
+  if (t.dim() == 4) ok = ok && t.stride(1) <= (1 << 24) - 128;  // sffft_linattn's token stride
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -105,7 +106,7 @@ Attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
               q.sizes(), ", ", k.sizes(), ", ", v.sizes());
   TORCH_CHECK(Dk >= 8 && Dv >= 8 && Dk <= 128 && Dv <= 128 && Dk % 8 == 0 && Dv % 8 == 0, LA,
               ": head channels must be multiples of 8 up to 128, got ", Dk, " and ", Dv);
-  TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX, LA, ": shape too large");
+  TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H * std::max(Dk, Dv) < (1 << 24), LA, ": shape too large");
   check_f32(LA, "log_decay", log_decay, q);
   TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == H, LA, ": log_decay must be [H] = [", H, "], got ",
               log_decay.sizes());
