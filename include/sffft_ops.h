@@ -34,7 +34,7 @@ extern "C" {
  * outside 0..T are taken as the nearest of these. */
 typedef struct sffft_linattn {
   int io;                 /* SFFFT_IO_F32 or SFFFT_IO_BF16: q, k, v, o and their gradients */
-  int B, T, H, Hk;        /* H a multiple of Hk */
+  int B, T, H, Hk;        /* H a multiple of Hk, at most 2^23 - 64 channels in all its heads */
   int Dk, Dv;             /* multiples of 8, at most 128 */
   float scale;
   long long q[3], k[3], v[3]; /* element strides (batch, token, head): multiples of 16 bytes, the token's

@@ -19,7 +19,8 @@ constexpr long long MAX_TOKEN_STRIDE = (1 << 24) - MAX_D;
 bool valid_shape(const sffft_linattn* p) {
   if (!p || !ops::valid_io(p->io) || p->B < 1 || p->T < 1 || p->H < 1 || p->Hk < 1 || p->H % p->Hk) return false;
   if (p->Dk < 8 || p->Dv < 8 || p->Dk > MAX_D || p->Dv > MAX_D || p->Dk % 8 || p->Dv % 8) return false;
-  return (long long)p->B * p->H <= INT_MAX / 64 && (long long)p->B * p->T <= INT_MAX;
+  return (long long)p->B * p->H <= INT_MAX / 64 && (long long)p->B * p->T <= INT_MAX &&
+         (long long)p->H * std::max(p->Dk, p->Dv) <= MAX_TOKEN_STRIDE / 2;
 }
 
 // A strided input: 16-byte aligned rows, and its extent.
@@ -48,20 +49,28 @@ Cut cut_of(const sffft_linattn* p, int marches) {
   return {(chunks + per - 1) / per, per * C};
 }
 
-template <class T, int KT, int VT, bool OUT>
+template <class T, class TO, int KT, int VT, bool OUT, int UP>
 hipError_t launch(la::Launch& L, hipStream_t st) {
   L.vtiles = 1;
   for (int i = 0; i < L.nm; i++) L.vtiles = std::max(L.vtiles, (L.m[i].V + VT - 1) / VT);
   const int units = L.s.B * L.s.H * L.nseg;
-  hipLaunchKernelGGL((la::march_kernel<T, KT, VT, OUT>), dim3((unsigned)((units + 7) / 8 * 8 * L.nm * L.vtiles)),
+  hipLaunchKernelGGL((la::march_kernel<T, TO, KT, VT, OUT, UP>), dim3((unsigned)((units + 7) / 8 * 8 * L.nm * L.vtiles)),
                      dim3(256), 0, st, L);
   return hipGetLastError();
 }
-// D: the most channels of any operand
-template <class T, bool OUT>
-hipError_t march(la::Launch L, int D, hipStream_t st) {
+template <class T, class TO, bool OUT, int UP>
+hipError_t march_planes(la::Launch& L, int D, hipStream_t st) {
   constexpr int VT = sizeof(T) == 4 ? 64 : 128;  // fp32: the planes of 128 columns leave no room for a second workgroup
-  return D > 64 ? launch<T, 128, VT, OUT>(L, st) : launch<T, 64, 64, OUT>(L, st);
+  return D > 64 ? launch<T, TO, 128, VT, OUT, UP>(L, st) : launch<T, TO, 64, 64, OUT, UP>(L, st);
+}
+// D: the most channels of any operand
+template <class T, bool OUT, class TO = T>
+hipError_t march(la::Launch L, int D, hipStream_t st) {
+  bool state = !OUT || sizeof(T) == 4;  // whether states leave in fp32
+  for (int i = 0; i < L.nm; i++) state = state || L.m[i].s1;
+  if constexpr (OUT && sizeof(T) == 2)
+    if (!state) return march_planes<T, TO, OUT, 2>(L, D, st);
+  return march_planes<T, TO, OUT, 3>(L, D, st);
 }
 hipError_t scan(const la::ScanLaunch& L, int n, hipStream_t st) {
   const unsigned tiles = (unsigned)((L.c[0].n + 1023) / 1024);
@@ -92,7 +101,7 @@ hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const v
   const Cut cut = cut_of(p, 1);
   const long long n = (long long)p->Dk * p->Dv;
   March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, n, 0, s1, n, 0,
-             p->Dk, p->Dv, p->Dv, 1, 0, 0, p->scale, p->scale, 1.f};
+             p->Dk, p->Dv, p->Dv, 1, 0, p->scale, p->scale, 1.f};
   la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1};
   if (cut.nseg > 1) {
     L.m[0].s0 = nullptr, L.m[0].s1 = work, L.m[0].s1_bh = n * cut.nseg, L.m[0].s1_seg = n;
@@ -119,20 +128,29 @@ hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const 
   hipError_t e = hipSuccess;
   if (cut.nseg > 1) {
     L.nm = 2;
-    L.m[0] = {Q, K, V, nullptr, nullptr, 0, 0, ws, ns, n, Dk, Dv, Dv, 1, 0, 0, c, c, 1.f};
-    L.m[1] = {K, Q, O, nullptr, nullptr, 0, 0, wd, ns, n, Dk, Dv, Dv, 1, 1, 0, c, 1.f, c};
+    L.m[0] = {Q, K, V, nullptr, nullptr, 0, 0, ws, ns, n, Dk, Dv, Dv, 1, 0, c, c, 1.f};
+    L.m[1] = {K, Q, O, nullptr, nullptr, 0, 0, wd, ns, n, Dk, Dv, Dv, 1, 1, c, 1.f, c};
     e = march<T, false>(L, D, st);
     if (e == hipSuccess)
       e = scan({{{ws, s0, nullptr, (int)n, 0}, {wd, ds1, ds0, (int)n, 1}}, s, cut.nseg, cut.seg}, 2, st);
     if (e != hipSuccess) return e;
     s0 = ws, ds1 = wd, ds0 = nullptr, L.nm = 3;
   }
-  L.m[0] = {O, V, K, dq, s0, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 0, 0, c, c, 1.f};
-  L.m[1] = {K, Q, O, G > 1 ? wv : dv, ds1, ns, nz, ds0, n, 0, Dk, Dv, Dv, 1, 1, G > 1, c, 1.f, c};
-  L.m[2] = {V, O, Q, G > 1 ? wk : dk, ds1, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 1, G > 1, c, 1.f, c};
-  e = march<T, true>(L, D, st);
-  if (e == hipSuccess && G > 1) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * Dk, Dk, G, st);
-  if (e == hipSuccess && G > 1) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * Dv, Dv, G, st);
+  const March mq = {O, V, K, dq, s0, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 0, c, c, 1.f};
+  const March mv = {K, Q, O, G > 1 ? wv : dv, ds1, ns, nz, ds0, n, 0, Dk, Dv, Dv, 1, 1, c, 1.f, c};
+  const March mk = {V, O, Q, G > 1 ? wk : dk, ds1, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 1, c, 1.f, c};
+  if (G == 1 || sizeof(T) == 4) {
+    L.m[0] = mq, L.m[1] = mv, L.m[2] = mk;
+    e = march<T, true>(L, D, st);
+    if (G == 1) return e;
+  } else {  // what is summed afterwards leaves in fp32: a launch of its own
+    L.nm = 1, L.m[0] = mq;
+    e = march<T, true>(L, D, st);
+    L.nm = 2, L.m[0] = mv, L.m[1] = mk;
+    if (e == hipSuccess) e = march<T, true, float>(L, D, st);
+  }
+  if (e == hipSuccess) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * Dk, Dk, G, st);
+  if (e == hipSuccess) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * Dv, Dv, G, st);
   return e;
 }
 

@@ -28,6 +28,7 @@ namespace la {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16;
 
@@ -44,13 +45,13 @@ struct Operand {
 // from the token on (the first one sees X0 undecayed, and the update includes the decay of the step).
 struct March {
   Operand a, b, c;
-  void* out;  // [B][T][H][V], in the operands' type, or fp32 if out_f32
+  void* out;  // [B][T][H][V]
   const float* s0;
   long long s0_bh, s0_seg;
   float* s1;
   long long s1_bh, s1_seg;
   int K, V, sk, sv;
-  int rev, out_f32;
+  int rev;
   float p, x, w;
 };
 
@@ -90,6 +91,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& h, uint32_t& 
   l = __builtin_amdgcn_perm(__float_as_uint(yl), __float_as_uint(xl), 0x07060302);
 }
 
+// x = h + m to 16 bits, each rounded
+__device__ __forceinline__ void split2(float x, float y, uint32_t& h, uint32_t& m) {
+  h = ops::pack_bf16(x, y);
+  m = ops::pack_bf16(x - __uint_as_float(h << 16), y - __uint_as_float(h & 0xffff0000u));
+}
+
 // NS planes of one operand fragment
 template <int NS>
 struct Frag {
@@ -105,6 +112,18 @@ __device__ __forceinline__ void product(const Frag<NA>& a, const Frag<NB>& b, f3
     for (int i = 0; i < NA; i++)
       if (s - i >= 0 && s - i < NB) d = mfma(a.p[i], b.p[s - i], d);
 }
+// the same for several accumulators at once: products that follow each other do not wait for each other
+template <int NA, int NB, int N, class FA, class FB, class FD>
+__device__ __forceinline__ void products(FA a, FB b, FD d) {
+  constexpr int LAST = (NA > NB ? NA : NB) - 1;
+#pragma unroll
+  for (int s = LAST; s >= 0; s--)
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+      if (s - i >= 0 && s - i < NB)
+#pragma unroll
+        for (int n = 0; n < N; n++) d(n) = mfma(a(n).p[i], b(n).p[s - i], d(n));
+}
 template <int NS>
 __device__ __forceinline__ Frag<NS> split8(const float (&x)[8]) {
   Frag<NS> f;
@@ -112,6 +131,12 @@ __device__ __forceinline__ Frag<NS> split8(const float (&x)[8]) {
     const uint4 v = make_uint4(ops::pack_bf16(x[0], x[1]), ops::pack_bf16(x[2], x[3]), ops::pack_bf16(x[4], x[5]),
                                ops::pack_bf16(x[6], x[7]));
     f.p[0] = __builtin_bit_cast(bf16x8, v);
+  } else if constexpr (NS == 2) {
+    uint32_t h[4], m[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], m[i]);
+    f.p[0] = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
+    f.p[1] = __builtin_bit_cast(bf16x8, make_uint4(m[0], m[1], m[2], m[3]));
   } else {
     uint32_t h[4], m[4], l[4];
 #pragma unroll
@@ -204,22 +229,29 @@ constexpr int chunk_of() { return sizeof(T) == 4 ? 32 : 64; }
 
 // Four wavefronts; wavefront w holds the columns vv = v0 + w VT/4 .. of the state, in the layout of an
 // accumulator (row kk = 16 a + 4 g + r, column lane % 16), which is an operand's too when the other operand
-// takes the same order of channels (rows_acc). With !OUT only the state is made.
-template <class T, int KT, int VT, bool OUT>
-__global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
-  constexpr int NS = sizeof(T) == 4 ? 3 : 1, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, VW = VT / 64;
-  constexpr int TILES = MT * (MT + 1) / 2, NP = (TILES + 3) / 4;
+// takes the same order of channels (rows_acc). With !OUT only the state is made. UP: the planes of what is
+// added to the state; 2 where it only serves outputs of 16 bits. TO: the output's type (fp32 for parts that are
+// summed).
+//
+// The next chunk is fetched a chunk ahead, and a chunk's outputs leave at the start of the next, before that
+// fetch: the wait for it then finds them gone.
+template <class T, class TO, int KT, int VT, bool OUT, int UP>
+__global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) {
+  constexpr int NS = sizeof(T) == 4 ? 3 : 1, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, KA = KT / 16;
+  constexpr int VW = VT / 64, TILES = MT * (MT + 1) / 2, NP = (TILES + 3) / 4;  // P's tiles, and those of a wavefront (some twice)
+  constexpr int E = sizeof(TO);
   __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, KT + 16> ta;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, KT + 16> tb;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, VT + 16> tc;
   __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, C + 8> tp;
+  __shared__ __attribute__((aligned(16))) float fi[C], wj[C];  // decays: of the entering state at row i, of token j in the update
 
   // Workgroups go to the 8 XCDs in turn; the marches and V tiles of one head and segment, which read the same
   // operands, follow each other on one of them.
   const int per = L.nm * L.vtiles, y = blockIdx.x >> 3;
   const int unit = y / per * 8 + (blockIdx.x & 7), sub = y % per;
   if (unit >= L.s.B * L.s.H * L.nseg) return;
-  const March& m = L.m[sub / L.vtiles];
+  const March m = L.m[sub / L.vtiles];
   const int v0 = sub % L.vtiles * VT;
   if (v0 >= m.V) return;
   const int h = unit % L.s.H, zb = unit / L.s.H, z = zb % L.nseg, b = zb / L.nseg;
@@ -228,61 +260,57 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool rev = m.rev;
   const int first = z * L.seg, last = min(first + L.seg, L.s.T), chunks = (last - first + C - 1) / C;
-  const int valid = valid_tokens(L.s, b);
+  const int end = min(valid_tokens(L.s, b), last);  // of the tokens that count
   const float l2 = decay_log2(L.s.log_decay, h);
-  auto power = [&](int n) { return n < 0 ? 0.f : exp2f(l2 * (float)n); };
+  auto power = [&](int n) { return n < 0 ? 0.f : __builtin_amdgcn_exp2f(l2 * (float)n); };
+  auto count = [&](int t0) { return __builtin_amdgcn_readfirstlane(min(max(end - t0, 0), C)); };
 
-  const T* pa = static_cast<const T*>(m.a.p) + b * m.a.sb + (h / m.a.div) * m.a.sh;
-  const T* pb = static_cast<const T*>(m.b.p) + b * m.b.sb + (h / m.b.div) * m.b.sh;
-  const T* pc = static_cast<const T*>(m.c.p) + b * m.c.sb + (h / m.c.div) * m.c.sh + v0;
+  // the first chunk: the last one of the segment if reversed
+  const int dir = rev ? -C : C;
+  int t0 = rev ? first + (chunks - 1) * C : first;
+  const T* pa = static_cast<const T*>(m.a.p) + b * m.a.sb + (h / m.a.div) * m.a.sh + t0 * m.a.st;
+  const T* pb = static_cast<const T*>(m.b.p) + b * m.b.sb + (h / m.b.div) * m.b.sh + t0 * m.b.st;
+  const T* pc = static_cast<const T*>(m.c.p) + b * m.c.sb + (h / m.c.div) * m.c.sh + t0 * m.c.st + v0;
+  const int orow = L.s.H * m.V;
+  TO* po = OUT ? static_cast<TO*>(m.out) + (((long long)b * L.s.T + t0) * L.s.H + h) * m.V : nullptr;
+
+  Stage<T, C, KT> ga, gb;
+  Stage<T, C, VT> gc;
+  auto fetch = [&](int n) {
+    if constexpr (OUT) ga.load(pa, m.a.st, n, m.K);
+    gb.load(pb, m.b.st, n, m.K);
+    gc.load(pc, m.c.st, n, m.V - v0);
+    pa += dir * m.a.st, pb += dir * m.b.st, pc += dir * m.c.st;
+  };
+  int n = count(t0);
+  fetch(n);
 
   // the wavefront's tiles of P: (row tile, column tile), and their decays
   int pi[NP], pj[NP];
   float pd[NP][4];
   if constexpr (OUT) {
 #pragma unroll
-    for (int n = 0; n < NP; n++) {
-      const int idx = w + 4 * n;
+    for (int t = 0; t < NP; t++) {
+      const int idx = min(w + 4 * t, TILES - 1);
       int r = 0;
       while ((r + 1) * (r + 2) / 2 <= idx) r++;
       const int c = idx - r * (r + 1) / 2;
-      pi[n] = __builtin_amdgcn_readfirstlane(rev ? c : r), pj[n] = __builtin_amdgcn_readfirstlane(rev ? r : c);
+      pi[t] = __builtin_amdgcn_readfirstlane(rev ? c : r), pj[t] = __builtin_amdgcn_readfirstlane(rev ? r : c);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int d = 16 * pi[n] + i16 - (16 * pj[n] + 4 * g + e);
-        pd[n][e] = m.p * power(rev ? -d : d);
+        const int d = 16 * pi[t] + i16 - (16 * pj[t] + 4 * g + e);
+        pd[t][e] = m.p * power(rev ? -d : d);
       }
     }
     // tiles on the other side of the diagonal stay zero
     for (int i = threadIdx.x; i < (int)sizeof(tp) / 16; i += 256) reinterpret_cast<uint4*>(&tp)[i] = make_uint4(0, 0, 0, 0);
   }
 
-  // decays that depend on the tokens in a chunk: of the rows that see the entering state, of the state, and of
-  // the tokens that are added to it
-  float fi[MT], gn, wj[JS][8];
-  int have = -1;
-  auto decays = [&](int n) {
-    have = n;
-    gn = power(n);
-#pragma unroll
-    for (int t = 0; t < MT; t++) {
-      const int i = 16 * t + i16;
-      fi[t] = m.x * (rev ? power(n - 1 - i) : power(i + 1));
-    }
-#pragma unroll
-    for (int s = 0; s < JS; s++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int j = 32 * s + 4 * g + (e & 3) + 16 * (e >> 2);
-        wj[s][e] = j < n ? m.w * power(rev ? j + 1 : n - 1 - j) : 0.f;
-      }
-  };
-
-  f32x4 S[KT / 16][VW];
+  f32x4 S[KA][VW];
   {
     const float* s0 = m.s0 ? m.s0 + bh * m.s0_bh + z * m.s0_seg : nullptr;
 #pragma unroll
-    for (int a = 0; a < KT / 16; a++)
+    for (int a = 0; a < KA; a++)
 #pragma unroll
       for (int v = 0; v < VW; v++)
 #pragma unroll
@@ -292,49 +320,101 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
         }
   }
 
-  Stage<T, C, KT> ga, gb;
-  Stage<T, C, VT> gc;
-  auto start = [&](int c) { return first + (rev ? chunks - 1 - c : c) * C; };
-  auto fetch = [&](int c) {
-    const int t0 = start(c), n = min(max(min(valid, last) - t0, 0), C);
-    if constexpr (OUT) ga.load(pa + t0 * m.a.st, m.a.st, n, m.K);
-    gb.load(pb + t0 * m.b.st, m.b.st, n, m.K);
-    gc.load(pc + t0 * m.c.st, m.c.st, n, m.V - v0);
+  // A chunk's outputs, transposed: rows vv, columns i. Where a's tile has their size they go through it, dead
+  // by then, so that whole rows leave together (a store of 4 channels in each of 16 rows takes the
+  // address unit 64 cycles, of 8 whole rows 16), each lane from the pieces that it will overwrite with the
+  // next chunk's a; rows from `left` on are not written.
+  constexpr bool VIA = OUT && NS == 1 && E == 2 && KT == VT;
+  f32x4 o[MT][VW] = {};
+  int left = 0;
+  auto stage_out = [&]() {
+    if constexpr (VIA)
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int v = 0; v < VW; v++)
+          *reinterpret_cast<uint2*>(&ta.v[0][16 * t + i16][16 * (w * VW + v) + 4 * g]) =
+              make_uint2(ops::pack_bf16(o[t][v][0], o[t][v][1]), ops::pack_bf16(o[t][v][2], o[t][v][3]));
   };
-  fetch(0);
+  auto store_out = [&]() {
+    if constexpr (VIA) {
+      typedef Stage<T, C, VT> G;
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(po + v0, 0, 0x7fffffff, 0x00027000);
+      const int row = threadIdx.x / G::PER, col = threadIdx.x % G::PER * G::E;
+      const uint32_t at = v0 + col < m.V ? (uint32_t)(row * orow + col) * E : 0x80000000u;
+#pragma unroll
+      for (int i = 0; i < G::N; i++) {
+        const i32x4 x = *reinterpret_cast<const i32x4*>(&ta.v[0][row + i * G::ROWS][col]);
+        __builtin_amdgcn_raw_buffer_store_b128(x, r, row + i * G::ROWS < left ? at : 0x80000000u, i * G::ROWS * orow * E, 0);
+      }
+    } else {
+      const auto r = __builtin_amdgcn_make_buffer_rsrc(po, 0, 0x7fffffff, 0x00027000);
+      const int ovv = v0 + 16 * w * VW + 4 * g;
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int v = 0; v < VW; v++) {
+          const bool in = (16 * t + i16 < left) & (ovv + 16 * v < m.V);
+          const uint32_t to = in ? (uint32_t)(i16 * orow + ovv) * E : 0x80000000u;
+          const int off = 16 * (t * orow + v) * E;
+          if constexpr (E == 2) {
+            const i32x2 x = {(int)ops::pack_bf16(o[t][v][0], o[t][v][1]), (int)ops::pack_bf16(o[t][v][2], o[t][v][3])};
+            __builtin_amdgcn_raw_buffer_store_b64(x, r, to, off, 0);
+          } else {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, o[t][v]), r, to, off, 0);
+          }
+        }
+    }
+  };
 
+  float gn = 1.f;
+  int have = -1;
   for (int c = 0; c < chunks; c++) {
-    const int t0 = start(c), n = min(max(min(valid, last) - t0, 0), C);
-    if (n != have) decays(n);
     __syncthreads();
-    if constexpr (OUT) ga.store(ta);
+    if constexpr (OUT) {  // the last chunk's
+      store_out();
+      if (c) po += (long long)dir * orow;
+      left = last - t0;
+      ga.store(ta);
+    }
     gb.store(tb);
     gc.store(tc);
-    if (c + 1 < chunks) fetch(c + 1);
+    if (n != have) {  // the decays depend on the tokens in a chunk
+      have = n;
+      gn = power(n);
+      const int i = threadIdx.x;
+      if (i < C) {
+        fi[i] = m.x * power(rev ? n - 1 - i : i + 1);
+        wj[i] = m.w * power(i >= n ? -1 : rev ? i + 1 : n - 1 - i);
+      }
+    }
+    t0 += dir;
+    n = c + 1 < chunks ? count(t0) : 0;  // past the last chunk nothing is valid, and nothing is read
+    fetch(n);
     __syncthreads();
 
-    f32x4 o[MT][VW];
     if constexpr (OUT) {
       // P^T tiles: rows j, columns i
 #pragma unroll
       for (int t = 0; t < NP; t++) {
-        if (w + 4 * t < TILES) {
-          f32x4 d = {0.f, 0.f, 0.f, 0.f};
+        Frag<NS> fb[KS], fa[KS];
 #pragma unroll
-          for (int k = 0; k < KS; k++) product(tb.rows(16 * pj[t], 32 * k, i16, g), ta.rows(16 * pi[t], 32 * k, i16, g), d);
-          // stored in the order of the transposing reads' rows: 16 * (j / 16 % 2) + 4 g + e at 8 g + 4 (j / 16 % 2) + e
-          u16* q = &tp.v[0][16 * pi[t] + i16][32 * (pj[t] >> 1) + 8 * g + 4 * (pj[t] & 1)];
-          const float x0 = d[0] * pd[t][0], x1 = d[1] * pd[t][1], x2 = d[2] * pd[t][2], x3 = d[3] * pd[t][3];
-          if constexpr (NS == 1) {
-            *reinterpret_cast<uint2*>(q) = make_uint2(ops::pack_bf16(x0, x1), ops::pack_bf16(x2, x3));
-          } else {
-            uint2 hh, mm, ll;
-            split2(x0, x1, hh.x, mm.x, ll.x);
-            split2(x2, x3, hh.y, mm.y, ll.y);
-            *reinterpret_cast<uint2*>(q) = hh;
-            *reinterpret_cast<uint2*>(q + C * (C + 8)) = mm;
-            *reinterpret_cast<uint2*>(q + 2 * C * (C + 8)) = ll;
-          }
+        for (int k = 0; k < KS; k++) fb[k] = tb.rows(16 * pj[t], 32 * k, i16, g), fa[k] = ta.rows(16 * pi[t], 32 * k, i16, g);
+        f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; k++) product(fb[k], fa[k], d);
+        // stored in the order of the transposing reads' rows: 16 * (j / 16 % 2) + 4 g + e at 8 g + 4 (j / 16 % 2) + e
+        u16* q = &tp.v[0][16 * pi[t] + i16][32 * (pj[t] >> 1) + 8 * g + 4 * (pj[t] & 1)];
+        const float x0 = d[0] * pd[t][0], x1 = d[1] * pd[t][1], x2 = d[2] * pd[t][2], x3 = d[3] * pd[t][3];
+        if constexpr (NS == 1) {
+          *reinterpret_cast<uint2*>(q) = make_uint2(ops::pack_bf16(x0, x1), ops::pack_bf16(x2, x3));
+        } else {
+          uint2 hh, mm, ll;
+          split2(x0, x1, hh.x, mm.x, ll.x);
+          split2(x2, x3, hh.y, mm.y, ll.y);
+          *reinterpret_cast<uint2*>(q) = hh;
+          *reinterpret_cast<uint2*>(q + C * (C + 8)) = mm;
+          *reinterpret_cast<uint2*>(q + 2 * C * (C + 8)) = ll;
         }
       }
       // a X, transposed: rows vv, columns i
@@ -344,7 +424,9 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
         for (int v = 0; v < VW; v++) o[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        Frag<NS> fs[VW];
+        Frag<NS> fs[VW], fa[MT];
+#pragma unroll
+        for (int t = 0; t < MT; t++) fa[t] = ta.rows_acc(16 * t, 32 * k, i16, g);
 #pragma unroll
         for (int v = 0; v < VW; v++) {
           float x[8];
@@ -352,87 +434,69 @@ __global__ __launch_bounds__(256, 2) void march_kernel(Launch L) {
           for (int e = 0; e < 8; e++) x[e] = S[2 * k + (e >> 2)][v][e & 3];
           fs[v] = split8<NS>(x);
         }
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-          const Frag<NS> fa = ta.rows_acc(16 * t, 32 * k, i16, g);
-#pragma unroll
-          for (int v = 0; v < VW; v++) product(fs[v], fa, o[t][v]);
-        }
+        products<NS, NS, MT * VW>([&](int n) -> auto& { return fs[n % VW]; }, [&](int n) -> auto& { return fa[n / VW]; },
+                                  [&](int n) -> auto& { return o[n / VW][n % VW]; });
       }
 #pragma unroll
-      for (int t = 0; t < MT; t++)
+      for (int t = 0; t < MT; t++) {
+        const float f = fi[16 * t + i16];
 #pragma unroll
-        for (int v = 0; v < VW; v++) o[t][v] *= fi[t];
+        for (int v = 0; v < VW; v++) o[t][v] *= f;
+      }
       __syncthreads();
     }
 
-    // c's channels as an operand, tokens along the sum
-    Frag<NS> fc[JS][VW];
 #pragma unroll
-    for (int s = 0; s < JS; s++)
-#pragma unroll
-      for (int v = 0; v < VW; v++) fc[s][v] = tc.cols(32 * s, 16 * (w * VW + v), i16, g);
-    if constexpr (OUT) {
-#pragma unroll
-      for (int s = 0; s < JS; s++)
-#pragma unroll
-        for (int t = 0; t < MT; t++)
-          if (rev ? 2 * s + 1 >= t : 2 * s <= t) {
-            const Frag<NS> fp = tp.rows(16 * t, 32 * s, i16, g);
-#pragma unroll
-            for (int v = 0; v < VW; v++) product(fc[s][v], fp, o[t][v]);
-          }
-#pragma unroll
-      for (int t = 0; t < MT; t++) {
-        const int tok = t0 + 16 * t + i16;
-        if (tok < last) {
-#pragma unroll
-          for (int v = 0; v < VW; v++) {
-            const int vv = v0 + 16 * (w * VW + v) + 4 * g;
-            if (vv < m.V) {
-              const long long at = (((long long)b * L.s.T + tok) * L.s.H + h) * m.V + vv;
-              const float x[4] = {o[t][v][0], o[t][v][1], o[t][v][2], o[t][v][3]};
-              if (m.out_f32) ops::store(static_cast<float*>(m.out) + at, x);
-              else ops::store(static_cast<T*>(m.out) + at, x);
-            }
-          }
-        }
-      }
-    }
-
-    // the state: decayed, and the chunk's tokens added
-#pragma unroll
-    for (int a = 0; a < KT / 16; a++)
+    for (int a = 0; a < KA; a++)
 #pragma unroll
       for (int v = 0; v < VW; v++) S[a][v] *= gn;
 #pragma unroll
     for (int s = 0; s < JS; s++) {
-      Frag<3> fw[VW];
+      // c's channels as an operand, tokens along the sum; and decayed, to be added to the state
+      Frag<NS> fc[VW];
+      Frag<UP> fw[VW];
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(&wj[32 * s + 4 * g]), w1 = *reinterpret_cast<const f32x4*>(&wj[32 * s + 16 + 4 * g]);
 #pragma unroll
       for (int v = 0; v < VW; v++) {
+        fc[v] = tc.cols(32 * s, 16 * (w * VW + v), i16, g);
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          x[e] = 0.f;
+          x[e] = (float)fc[v].p[NS - 1][e];
 #pragma unroll
-          for (int p = NS - 1; p >= 0; p--) x[e] += (float)fc[s][v].p[p][e];
-          x[e] *= wj[s][e];
+          for (int p = NS - 2; p >= 0; p--) x[e] += (float)fc[v].p[p][e];
+          x[e] *= e < 4 ? w0[e & 3] : w1[e & 3];
         }
-        fw[v] = split8<3>(x);
+        fw[v] = split8<UP>(x);
       }
+      if constexpr (OUT) {
+        Frag<NS> fp[MT];  // the zero tiles too: their two products cost less than branches
 #pragma unroll
-      for (int a = 0; a < KT / 16; a++) {
-        const Frag<NS> fb = tb.cols(32 * s, 16 * a, i16, g);
+        for (int t = 0; t < MT; t++) fp[t] = tp.rows(16 * t, 32 * s, i16, g);
+        products<NS, NS, MT * VW>([&](int n) -> auto& { return fc[n % VW]; }, [&](int n) -> auto& { return fp[n / VW]; },
+                                  [&](int n) -> auto& { return o[n / VW][n % VW]; });
+      }
+      constexpr int HALF = 2;
 #pragma unroll
-        for (int v = 0; v < VW; v++) product(fb, fw[v], S[a][v]);
+      for (int a = 0; a < KA; a += HALF) {
+        Frag<NS> fb[HALF];
+#pragma unroll
+        for (int i = 0; i < HALF; i++) fb[i] = tb.cols(32 * s, 16 * (a + i), i16, g);
+        products<NS, UP, HALF * VW>([&](int n) -> auto& { return fb[n / VW]; }, [&](int n) -> auto& { return fw[n % VW]; },
+                                    [&](int n) -> auto& { return S[a + n / VW][n % VW]; });
       }
     }
+    if constexpr (OUT) stage_out();
+  }
+  if constexpr (OUT) {
+    if constexpr (VIA) __syncthreads();
+    store_out();
   }
 
   if (m.s1) {
     float* s1 = m.s1 + bh * m.s1_bh + z * m.s1_seg;
 #pragma unroll
-    for (int a = 0; a < KT / 16; a++)
+    for (int a = 0; a < KA; a++)
 #pragma unroll
       for (int v = 0; v < VW; v++)
 #pragma unroll

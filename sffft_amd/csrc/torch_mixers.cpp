@@ -106,7 +106,7 @@ Attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, const 
               q.sizes(), ", ", k.sizes(), ", ", v.sizes());
   TORCH_CHECK(Dk >= 8 && Dv >= 8 && Dk <= 128 && Dv <= 128 && Dk % 8 == 0 && Dv % 8 == 0, LA,
               ": head channels must be multiples of 8 up to 128, got ", Dk, " and ", Dv);
-  TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H * std::max(Dk, Dv) < (1 << 24), LA, ": shape too large");
+  TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && H * std::max(Dk, Dv) <= (1 << 23) - 64, LA, ": shape too large");
   check_f32(LA, "log_decay", log_decay, q);
   TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == H, LA, ": log_decay must be [H] = [", H, "], got ",
               log_decay.sizes());
