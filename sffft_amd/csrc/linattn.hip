@@ -53,7 +53,7 @@ template <class T, class TO, int KT, int VT, bool OUT, int UP>
 hipError_t launch(la::Launch& L, hipStream_t st) {
   L.vtiles = 1;
   for (int i = 0; i < L.nm; i++) L.vtiles = std::max(L.vtiles, (L.m[i].V + VT - 1) / VT);
-  const int units = L.s.B * L.s.H * L.nseg;
+  const int units = L.s.B * L.s.H * (OUT ? L.nseg : L.nseg - 1);
   hipLaunchKernelGGL((la::march_kernel<T, TO, KT, VT, OUT, UP>), dim3((unsigned)((units + 7) / 8 * 8 * L.nm * L.vtiles)),
                      dim3(256), 0, st, L);
   return hipGetLastError();
@@ -85,10 +85,12 @@ hipError_t head_sum(const float* in, void* out, long long n, int D, int G, hipSt
   return hipGetLastError();
 }
 
-// The segments' states
+// The segments' sums, or entering states
 size_t state_bytes(const sffft_linattn* p, const Cut& c) {
   return c.nseg == 1 ? 0 : (size_t)p->B * p->H * c.nseg * p->Dk * p->Dv * 4;
 }
+// More segments than this are joined by a launch of its own, fewer by each workgroup that follows them.
+constexpr int MAX_JOINED = 8;
 // dk and dv of heads that are shared, for each query head, before their sum
 size_t shared_bytes(const sffft_linattn* p) {
   return p->H == p->Hk ? 0 : (size_t)p->B * p->T * p->H * (p->Dk + p->Dv) * 4;
@@ -99,18 +101,13 @@ hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const v
                    const float* s0, void* o, float* s1, float* work, hipStream_t st) {
   const int G = p->H / p->Hk, D = std::max(p->Dk, p->Dv);
   const Cut cut = cut_of(p, 1);
-  const long long n = (long long)p->Dk * p->Dv;
-  March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, n, 0, s1, n, 0,
-             p->Dk, p->Dv, p->Dv, 1, 0, p->scale, p->scale, 1.f};
-  la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1};
-  if (cut.nseg > 1) {
-    L.m[0].s0 = nullptr, L.m[0].s1 = work, L.m[0].s1_bh = n * cut.nseg, L.m[0].s1_seg = n;
-    hipError_t e = march<T, false>(L, D, st);
-    if (e == hipSuccess) e = scan({{{work, s0, s1, (int)n, 0}}, s, cut.nseg, cut.seg}, 1, st);
-    if (e != hipSuccess) return e;
-    L.m[0] = m, L.m[0].s0 = work, L.m[0].s0_bh = n * cut.nseg, L.m[0].s0_seg = n, L.m[0].s1 = nullptr;
-  }
-  return march<T, true>(L, D, st);
+  const March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, work, s1, p->Dk, p->Dv, p->Dv, 1,
+                   0, p->scale, p->scale, 1.f};
+  const la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1, cut.nseg > MAX_JOINED};
+  hipError_t e = hipSuccess;
+  if (cut.nseg > 1) e = march<T, false>(L, D, st);
+  if (e == hipSuccess && L.scanned) e = scan({{{work, s0, p->Dk * p->Dv, 0}}, s, cut.nseg, cut.seg}, 1, st);
+  return e == hipSuccess ? march<T, true>(L, D, st) : e;
 }
 
 template <class T>
@@ -121,24 +118,20 @@ hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const 
   const Operand Q = operand(q, p->q, 1), K = operand(k, p->k, G), V = operand(v, p->v, G), O = operand(go, p->go, 1);
   const size_t rows = (size_t)p->B * p->T;
   const Cut cut = cut_of(p, 3);
-  const long long n = (long long)Dk * Dv, ns = cut.nseg > 1 ? n * cut.nseg : n, nz = cut.nseg > 1 ? n : 0;
-  float *ws = work, *wd = ws + state_bytes(p, cut) / 4, *wk = wd + state_bytes(p, cut) / 4, *wv = wk + rows * p->H * Dk;
+  const size_t states = state_bytes(p, cut) / 4;
+  float *ws = work, *wd = ws + states, *wk = wd + states, *wv = wk + rows * p->H * Dk;
   const float c = p->scale;
-  la::Launch L = {{}, s, 3, cut.nseg, cut.seg, 1};
+  const March mv = {K, Q, O, G > 1 ? wv : dv, ds1, wd, ds0, Dk, Dv, Dv, 1, 1, c, 1.f, c};
+  la::Launch L = {{{Q, K, V, nullptr, s0, ws, nullptr, Dk, Dv, Dv, 1, 0, c, c, 1.f}, mv}, s, 2, cut.nseg, cut.seg, 1,
+                  cut.nseg > MAX_JOINED};
   hipError_t e = hipSuccess;
-  if (cut.nseg > 1) {
-    L.nm = 2;
-    L.m[0] = {Q, K, V, nullptr, nullptr, 0, 0, ws, ns, n, Dk, Dv, Dv, 1, 0, c, c, 1.f};
-    L.m[1] = {K, Q, O, nullptr, nullptr, 0, 0, wd, ns, n, Dk, Dv, Dv, 1, 1, c, 1.f, c};
-    e = march<T, false>(L, D, st);
-    if (e == hipSuccess)
-      e = scan({{{ws, s0, nullptr, (int)n, 0}, {wd, ds1, ds0, (int)n, 1}}, s, cut.nseg, cut.seg}, 2, st);
-    if (e != hipSuccess) return e;
-    s0 = ws, ds1 = wd, ds0 = nullptr, L.nm = 3;
-  }
-  const March mq = {O, V, K, dq, s0, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 0, c, c, 1.f};
-  const March mv = {K, Q, O, G > 1 ? wv : dv, ds1, ns, nz, ds0, n, 0, Dk, Dv, Dv, 1, 1, c, 1.f, c};
-  const March mk = {V, O, Q, G > 1 ? wk : dk, ds1, ns, nz, nullptr, 0, 0, Dv, Dk, 1, Dv, 1, c, 1.f, c};
+  if (cut.nseg > 1) e = march<T, false>(L, D, st);
+  if (e == hipSuccess && L.scanned)
+    e = scan({{{ws, s0, Dk * Dv, 0}, {wd, ds1, Dk * Dv, 1}}, s, cut.nseg, cut.seg}, 2, st);
+  if (e != hipSuccess) return e;
+  L.nm = 3;
+  const March mq = {O, V, K, dq, s0, ws, nullptr, Dv, Dk, 1, Dv, 0, c, c, 1.f};
+  const March mk = {V, O, Q, G > 1 ? wk : dk, ds1, wd, nullptr, Dv, Dk, 1, Dv, 1, c, 1.f, c};
   if (G == 1 || sizeof(T) == 4) {
     L.m[0] = mq, L.m[1] = mv, L.m[2] = mk;
     e = march<T, true>(L, D, st);

@@ -39,17 +39,17 @@ struct Operand {
   int div;
 };
 
-// One march. State element (kk, vv) of (b, h) in segment z is at s[(b * H + h) * s_bh + z * s_seg + kk * sk
-// + vv * sv]. The update adds w b c^T; the products with the entering state take x, those within
+// One march. A state of (b, h) is an array [K][V] with element strides sk, sv: the one it starts from at
+// s0 + (b * H + h) * K * V, the sum of segment z alone at sums + ((b * H + h) * nseg + z) * K * V. A segment starts from s0,
+// decayed, and the sums of those before it (from the last one on if reversed); where there are many a scan has
+// put the entering states in the sums' place (scanned). s1 gets the state after the last segment. The update adds w b c^T; the products with the entering state take x, those within
 // the march p. Forward, the state enters before a token's own update (a_0 sees g X0); reversed, it holds all
 // from the token on (the first one sees X0 undecayed, and the update includes the decay of the step).
 struct March {
   Operand a, b, c;
   void* out;  // [B][T][H][V]
   const float* s0;
-  long long s0_bh, s0_seg;
-  float* s1;
-  long long s1_bh, s1_seg;
+  float *sums, *s1;
   int K, V, sk, sv;
   int rev;
   float p, x, w;
@@ -61,11 +61,12 @@ struct Shape {
   const int* lengths;
 };
 
-// A launch: nm marches over B * H heads, nseg segments of seg tokens, vtiles tiles of the V channels.
+// A launch: nm marches over B * H heads, nseg segments of seg tokens, vtiles tiles of the V channels. The sums are
+// made of all segments but the last of a march (the first if reversed).
 struct Launch {
   March m[3];
   Shape s;
-  int nm, nseg, seg, vtiles;
+  int nm, nseg, seg, vtiles, scanned;
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -250,11 +251,12 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   // operands, follow each other on one of them.
   const int per = L.nm * L.vtiles, y = blockIdx.x >> 3;
   const int unit = y / per * 8 + (blockIdx.x & 7), sub = y % per;
-  if (unit >= L.s.B * L.s.H * L.nseg) return;
+  const int segments = OUT ? L.nseg : L.nseg - 1;
+  if (unit >= L.s.B * L.s.H * segments) return;
   const March m = L.m[sub / L.vtiles];
   const int v0 = sub % L.vtiles * VT;
   if (v0 >= m.V) return;
-  const int h = unit % L.s.H, zb = unit / L.s.H, z = zb % L.nseg, b = zb / L.nseg;
+  const int h = unit % L.s.H, zb = unit / L.s.H, b = zb / segments, z = zb % segments + (!OUT && m.rev);
   const long long bh = (long long)b * L.s.H + h;
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -307,17 +309,58 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   }
 
   f32x4 S[KA][VW];
-  {
-    const float* s0 = m.s0 ? m.s0 + bh * m.s0_bh + z * m.s0_seg : nullptr;
+  const int kv = m.K * m.V, sv0 = v0 + 16 * w * VW + i16;
+  const uint32_t sat = (uint32_t)(4 * g * m.sk + sv0 * m.sv) * 4;
+  // f(tile, lane offset, scalar offset) for the tiles of a state; the lanes outside it get an offset outside
+  auto state_tiles = [&](auto f) {
 #pragma unroll
     for (int a = 0; a < KA; a++)
 #pragma unroll
-      for (int v = 0; v < VW; v++)
+      for (int v = 0; v < VW; v++) {
+        const bool in = (16 * a + 4 * g < m.K) & (sv0 + 16 * v < m.V);
+        f(a, v, in ? sat : 0x80000000u, (16 * a * m.sk + 16 * v * m.sv) * 4);
+      }
+  };
+  auto load_state = [&](const float* p, f32x4(&x)[KA][VW]) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, 0x7fffffff, 0x00027000);
+    if (m.sk == 1)  // rows kk next to each other
+      state_tiles([&](int a, int v, uint32_t at, int off) {
+        x[a][v] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, off, 0));
+      });
+    else
+      state_tiles([&](int a, int v, uint32_t at, int off) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int kk = 16 * a + 4 * g + r, vv = v0 + 16 * (w * VW + v) + i16;
-          S[a][v][r] = s0 && kk < m.K && vv < m.V ? s0[(long long)kk * m.sk + (long long)vv * m.sv] : 0.f;
-        }
+        for (int e = 0; e < 4; e++) x[a][v][e] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, off + e * m.sk * 4, 0));
+      });
+  };
+  auto store_state = [&](float* p) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00027000);
+    state_tiles([&](int a, int v, uint32_t at, int off) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(S[a][v][e]), r, at, off + e * m.sk * 4, 0);
+    });
+  };
+#pragma unroll
+  for (int a = 0; a < KA; a++)
+#pragma unroll
+    for (int v = 0; v < VW; v++) S[a][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (OUT) {
+    const float* sums = m.sums + bh * L.nseg * kv;
+    if (L.scanned) {
+      load_state(sums + (long long)z * kv, S);
+    } else {
+      if (m.s0) load_state(m.s0 + bh * kv, S);
+      const int total = valid_tokens(L.s, b);
+      for (int y = rev ? L.nseg - 1 : 0; y != z; y += rev ? -1 : 1) {
+        f32x4 u[KA][VW];
+        load_state(sums + (long long)y * kv, u);
+        const float d = power(min(max(total - y * L.seg, 0), L.seg));
+#pragma unroll
+        for (int a = 0; a < KA; a++)
+#pragma unroll
+          for (int v = 0; v < VW; v++) S[a][v] = S[a][v] * d + u[a][v];
+      }
+    }
   }
 
   // A chunk's outputs, transposed: rows vv, columns i. Where a's tile has their size they go through it, dead
@@ -493,26 +536,15 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
     store_out();
   }
 
-  if (m.s1) {
-    float* s1 = m.s1 + bh * m.s1_bh + z * m.s1_seg;
-#pragma unroll
-    for (int a = 0; a < KA; a++)
-#pragma unroll
-      for (int v = 0; v < VW; v++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int kk = 16 * a + 4 * g + r, vv = v0 + 16 * (w * VW + v) + i16;
-          if (kk < m.K && vv < m.V) s1[(long long)kk * m.sk + (long long)vv * m.sv] = S[a][v][r];
-        }
-  }
+  if constexpr (!OUT) store_state(m.sums + (bh * L.nseg + z) * kv);
+  else if (m.s1 && z == (rev ? 0 : L.nseg - 1)) store_state(m.s1 + bh * kv);
 }
 
-// The states that enter the segments, from those that the segments make of nothing, in place; and the last one.
-// Lane: four elements. Sixteen segments are read ahead.
+// The states that enter the segments, from the sums of those before them, in place. Lane: four elements. Sixteen
+// segments are read ahead.
 struct Scan {
-  float* seg;  // [bh][nseg][n]
+  float* sums;  // [bh][nseg][n]
   const float* s0;
-  float* s1;
   int n, rev;
 };
 struct ScanLaunch {
@@ -528,24 +560,23 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
   const float l2 = decay_log2(L.s.log_decay, h);
   float x[4] = {0.f, 0.f, 0.f, 0.f};
   if (c.s0) ops::load(c.s0 + (long long)bh * c.n + e, x);
-  float* p = c.seg + (long long)bh * L.nseg * c.n + e;
+  float* p = c.sums + (long long)bh * L.nseg * c.n + e;
   constexpr int AHEAD = 16;
   for (int z0 = 0; z0 < L.nseg; z0 += AHEAD) {
     float u[AHEAD][4];
 #pragma unroll
     for (int i = 0; i < AHEAD; i++)
-      if (z0 + i < L.nseg) ops::load(p + (long long)(c.rev ? L.nseg - 1 - z0 - i : z0 + i) * c.n, u[i]);
+      if (z0 + i < L.nseg - 1) ops::load(p + (long long)(c.rev ? L.nseg - 1 - z0 - i : z0 + i) * c.n, u[i]);
 #pragma unroll
     for (int i = 0; i < AHEAD; i++)
       if (z0 + i < L.nseg) {
         const int z = c.rev ? L.nseg - 1 - z0 - i : z0 + i;
-        const float d = exp2f(l2 * (float)min(max(valid - z * L.seg, 0), L.seg));
+        const float d = __builtin_amdgcn_exp2f(l2 * (float)min(max(valid - z * L.seg, 0), L.seg));
         ops::store(p + (long long)z * c.n, x);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = x[k] * d + u[i][k];
       }
   }
-  if (c.s1) ops::store(c.s1 + (long long)bh * c.n + e, x);
 }
 
 // Sum over the query heads that share a key/value head: out [rows][Hk][D] from in [rows][H][D].
