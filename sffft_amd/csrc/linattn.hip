@@ -1,6 +1,7 @@
 // Launches and C ABI of linear attention (linattn.hpp).
 #include <algorithm>
 #include <climits>
+#include <initializer_list>
 
 #include "linattn.hpp"
 #include "ops_status.hpp"
@@ -58,19 +59,23 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
                      dim3(256), 0, st, L);
   return hipGetLastError();
 }
+// Tiles of 64 or 128 channels. fp32 takes 64 of V: the planes of 128 leave no room for a second workgroup on a CU.
 template <class T, class TO, bool OUT, int UP>
-hipError_t march_planes(la::Launch& L, int D, hipStream_t st) {
-  constexpr int VT = sizeof(T) == 4 ? 64 : 128;  // fp32: the planes of 128 columns leave no room for a second workgroup
-  return D > 64 ? launch<T, TO, 128, VT, OUT, UP>(L, st) : launch<T, TO, 64, 64, OUT, UP>(L, st);
+hipError_t march_planes(la::Launch& L, hipStream_t st) {
+  const int K = L.m[0].K, V = L.m[0].V;
+  if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
+  if constexpr (sizeof(T) == 2)
+    if (V > 64) return launch<T, TO, 128, 128, OUT, UP>(L, st);
+  return launch<T, TO, 128, 64, OUT, UP>(L, st);
 }
-// D: the most channels of any operand
+// nm marches of the same K and V
 template <class T, bool OUT, class TO = T>
-hipError_t march(la::Launch L, int D, hipStream_t st) {
+hipError_t march(la::Launch L, hipStream_t st) {
   bool state = !OUT || sizeof(T) == 4;  // whether states leave in fp32
   for (int i = 0; i < L.nm; i++) state = state || L.m[i].s1;
   if constexpr (OUT && sizeof(T) == 2)
-    if (!state) return march_planes<T, TO, OUT, 2>(L, D, st);
-  return march_planes<T, TO, OUT, 3>(L, D, st);
+    if (!state) return march_planes<T, TO, OUT, 2>(L, st);
+  return march_planes<T, TO, OUT, 3>(L, st);
 }
 hipError_t scan(const la::ScanLaunch& L, int n, hipStream_t st) {
   const unsigned tiles = (unsigned)((L.c[0].n + 1023) / 1024);
@@ -99,22 +104,22 @@ size_t shared_bytes(const sffft_linattn* p) {
 template <class T>
 hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const void* v, const Shape& s,
                    const float* s0, void* o, float* s1, float* work, hipStream_t st) {
-  const int G = p->H / p->Hk, D = std::max(p->Dk, p->Dv);
+  const int G = p->H / p->Hk;
   const Cut cut = cut_of(p, 1);
   const March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, work, s1, p->Dk, p->Dv, p->Dv, 1,
                    0, p->scale, p->scale, 1.f};
   const la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1, cut.nseg > MAX_JOINED};
   hipError_t e = hipSuccess;
-  if (cut.nseg > 1) e = march<T, false>(L, D, st);
+  if (cut.nseg > 1) e = march<T, false>(L, st);
   if (e == hipSuccess && L.scanned) e = scan({{{work, s0, p->Dk * p->Dv, 0}}, s, cut.nseg, cut.seg}, 1, st);
-  return e == hipSuccess ? march<T, true>(L, D, st) : e;
+  return e == hipSuccess ? march<T, true>(L, st) : e;
 }
 
 template <class T>
 hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const void* v, const void* go,
                     const Shape& s, const float* s0, const float* ds1, void* dq, void* dk, void* dv, float* ds0,
                     float* work, hipStream_t st) {
-  const int G = p->H / p->Hk, D = std::max(p->Dk, p->Dv), Dk = p->Dk, Dv = p->Dv;
+  const int G = p->H / p->Hk, Dk = p->Dk, Dv = p->Dv;
   const Operand Q = operand(q, p->q, 1), K = operand(k, p->k, G), V = operand(v, p->v, G), O = operand(go, p->go, 1);
   const size_t rows = (size_t)p->B * p->T;
   const Cut cut = cut_of(p, 3);
@@ -125,23 +130,27 @@ hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const 
   la::Launch L = {{{Q, K, V, nullptr, s0, ws, nullptr, Dk, Dv, Dv, 1, 0, c, c, 1.f}, mv}, s, 2, cut.nseg, cut.seg, 1,
                   cut.nseg > MAX_JOINED};
   hipError_t e = hipSuccess;
-  if (cut.nseg > 1) e = march<T, false>(L, D, st);
+  if (cut.nseg > 1) e = march<T, false>(L, st);
   if (e == hipSuccess && L.scanned)
     e = scan({{{ws, s0, Dk * Dv, 0}, {wd, ds1, Dk * Dv, 1}}, s, cut.nseg, cut.seg}, 2, st);
   if (e != hipSuccess) return e;
-  L.nm = 3;
   const March mq = {O, V, K, dq, s0, ws, nullptr, Dv, Dk, 1, Dv, 0, c, c, 1.f};
   const March mk = {V, O, Q, G > 1 ? wk : dk, ds1, wd, nullptr, Dv, Dk, 1, Dv, 1, c, 1.f, c};
-  if (G == 1 || sizeof(T) == 4) {
-    L.m[0] = mq, L.m[1] = mv, L.m[2] = mk;
-    e = march<T, true>(L, D, st);
-    if (G == 1) return e;
-  } else {  // what is summed afterwards leaves in fp32: a launch of its own
-    L.nm = 1, L.m[0] = mq;
-    e = march<T, true>(L, D, st);
-    L.nm = 2, L.m[0] = mv, L.m[1] = mk;
-    if (e == hipSuccess) e = march<T, true, float>(L, D, st);
+  // One launch where the sizes and the types of the outputs are equal: what is summed afterwards leaves in fp32.
+  const auto run = [&](std::initializer_list<March> ms, bool parts) {
+    L.nm = 0;
+    for (const March& m : ms) L.m[L.nm++] = m;
+    if (e == hipSuccess) e = parts ? march<T, true, float>(L, st) : march<T, true>(L, st);
+  };
+  const bool parts = G > 1, split = parts && sizeof(T) == 2;
+  if (Dk == Dv) {
+    if (!split) run({mq, mv, mk}, false);
+    else run({mq}, false), run({mv, mk}, true);
+  } else {
+    if (!split) run({mq, mk}, false), run({mv}, false);
+    else run({mq}, false), run({mk}, true), run({mv}, true);
   }
+  if (!parts) return e;
   if (e == hipSuccess) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * Dk, Dk, G, st);
   if (e == hipSuccess) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * Dv, Dv, G, st);
   return e;
