@@ -72,7 +72,7 @@ int sffft_linattn_step(const sffft_linattn* p, const void* q, const void* k, con
  * interleaved:  a' = a cos - b sin,  b' = b cos + a sin; channels from R on are copied. With
  * inverse = 1 by the negative angle (the gradient). Token t of sequence b has position
  * pos[b][t] (pos_bits 32 or 64), t if pos is NULL; a position outside the table gives NaN in the
- * rotated channels and reads nothing. qo may be q and ko k, with equal strides; else they overlap
+ * rotated channels and reads nothing. (H + Hk) * D / 2 is at most 65535. qo may be q and ko k, with equal strides; else they overlap
  * neither. */
 typedef struct sffft_rotary {
   int io;

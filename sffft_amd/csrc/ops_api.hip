@@ -26,15 +26,20 @@ namespace {
 
 // ---- rotary ----
 
+// Vectors of 16 bytes where everything is aligned to them, else channel by channel. About one unit for each of a
+// workgroup's 256 lanes.
 template <class T>
-hipError_t rotary(rot::Args a, long long tokens, bool interleaved, bool wide, hipStream_t st) {
-  constexpr int PP = 16 / sizeof(T);
-  const int pp = wide ? PP : 1;
-  a.items = tokens * a.heads * (a.D / (2 * pp));
-  const dim3 grid((unsigned)((a.items + 255) / 256)), block(256);
+hipError_t rotary(rot::Args a, bool interleaved, bool wide, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const int pp = !wide ? 1 : interleaved ? V / 2 : V;
+  a.units = a.D / (2 * pp), a.per = a.heads * a.units;
+  const auto inverse = [](unsigned d) { return (unsigned)((((unsigned long long)1 << 32) + d - 1) / d); };
+  a.by_units = inverse(a.units), a.by_per = inverse(a.per);
+  a.wg_tokens = std::max(1u, 256u / a.per);
+  const dim3 grid((a.tokens + a.wg_tokens - 1) / a.wg_tokens), block(256);
   if (wide) {
-    if (interleaved) hipLaunchKernelGGL((rot::rotary_kernel<T, PP, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((rot::rotary_kernel<T, PP, false>), grid, block, 0, st, a);
+    if (interleaved) hipLaunchKernelGGL((rot::rotary_kernel<T, V / 2, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rot::rotary_kernel<T, V, false>), grid, block, 0, st, a);
   } else {
     if (interleaved) hipLaunchKernelGGL((rot::rotary_kernel<T, 1, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((rot::rotary_kernel<T, 1, false>), grid, block, 0, st, a);
@@ -161,8 +166,8 @@ int sffft_rotary_apply(const sffft_rotary* p, const void* q, const void* k, cons
       (p->Hk > 0) != (k != nullptr) || (p->Hk > 0) != (ko != nullptr))
     return SFFFT_EINVAL;
   const int elem = p->io ? 2 : 4;
-  const __int128 items = (__int128)p->B * p->T * ((__int128)p->H + p->Hk) * (p->D / 2);
-  if (items > (__int128)INT_MAX * 128 || (long long)p->H + p->Hk > INT_MAX) return SFFFT_EINVAL;
+  // a token's pairs are counted in 16 bits, the tokens in 31
+  if ((long long)p->B * p->T > INT_MAX || ((long long)p->H + p->Hk) * (p->D / 2) > 65535) return SFFFT_EINVAL;
   const size_t nq = ops::extent(p->q, p->B, p->T, p->H, p->D, elem), mq = ops::extent(p->qo, p->B, p->T, p->H, p->D, elem);
   const size_t nk = k ? ops::extent(p->k, p->B, p->T, p->Hk, p->D, elem) : 1;
   const size_t mk = k ? ops::extent(p->ko, p->B, p->T, p->Hk, p->D, elem) : 1;
@@ -182,7 +187,11 @@ int sffft_rotary_apply(const sffft_rotary* p, const void* q, const void* k, cons
   a.q = {q, qo, p->q[0], p->q[1], p->q[2], p->qo[0], p->qo[1], p->qo[2]};
   a.k = {k, ko, p->k[0], p->k[1], p->k[2], p->ko[0], p->ko[1], p->ko[2]};
   a.table = table, a.pos = pos, a.pos64 = p->pos_bits == 64, a.positions = p->positions;
-  a.T = p->T, a.H = p->H, a.heads = p->H + p->Hk, a.D = p->D, a.R = p->R, a.inverse = p->inverse;
+  a.tokens = (unsigned)((long long)p->B * p->T), a.T = p->T;
+  bool flat = pos || p->B == 1;  // one stride leads through all tokens, and no token's place in its sequence matters
+  for (const long long* s : {p->q, p->k, p->qo, p->ko}) flat = flat && (p->B == 1 || s[0] == s[1] * p->T || (!k && (s == p->k || s == p->ko)));
+  if (flat) a.T = a.tokens;
+  a.H = p->H, a.heads = p->H + p->Hk, a.D = p->D, a.R = p->R, a.inverse = p->inverse;
   // 16-byte loads of 8 bf16 or 4 fp32 channels; a lane takes two
   bool wide = p->D % (32 / elem) == 0 && p->R % (32 / elem) == 0 && ops::aligned(q, 16) && ops::aligned(k, 16) &&
               ops::aligned(qo, 16) && ops::aligned(ko, 16) && ops::aligned(table, 16);
@@ -190,7 +199,7 @@ int sffft_rotary_apply(const sffft_rotary* p, const void* q, const void* k, cons
     wide = wide && p->q[i] * elem % 16 == 0 && p->qo[i] * elem % 16 == 0 &&
            (!k || (p->k[i] * elem % 16 == 0 && p->ko[i] * elem % 16 == 0));
   const auto run = p->io ? rotary<uint16_t> : rotary<float>;
-  return ops::hip_status(run(a, (long long)p->B * p->T, p->interleaved, wide, (hipStream_t)stream), "rotary launch");
+  return ops::hip_status(run(a, p->interleaved, wide, (hipStream_t)stream), "rotary launch");
 }
 
 int sffft_rotary_table(int positions, int R, double base, int scaling, double factor, int trained, double magnitude,

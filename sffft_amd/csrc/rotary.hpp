@@ -19,62 +19,77 @@ struct Args {
   const float* table;
   const void* pos;
   int pos64, positions;
-  int T, H, heads, D, R, inverse;  // heads: of q and k together
-  long long items;
+  unsigned tokens, T;  // T = tokens where one stride leads through all of them
+  int H, heads, D, R, inverse;  // heads: of q and k together
+  unsigned units, per, wg_tokens, by_units, by_per;  // units of a head, of a token; ceil(2^32 / units), ceil(2^32 / per)
 };
 
-// A lane takes PP pairs of one head of one token, or 2 PP of the channels that are copied.
+// n / d for n * d < 2^32, from m = ceil(2^32 / d)
+__device__ __forceinline__ unsigned divide(unsigned n, unsigned d, unsigned m) { return d == 1 ? n : __umulhi(n, m); }
+
+// A lane takes one unit of one head of one token: half layout, PP pairs in two vectors; interleaved, PP pairs in one;
+// of the channels that are copied as much. Neighbouring lanes take neighbouring vectors.
 template <class T, int PP, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void rotary_kernel(Args A) {
-  const int units = A.D / (2 * PP), turned = A.R / (2 * PP);
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= A.items) return;
-  const long long at = i / units, bt = at / A.heads;
-  const int u = (int)(i - at * units), head = (int)(at - bt * A.heads);
-  const long long b = bt / A.T;
-  const int t = (int)(bt - b * A.T);
-  const Side& s = head < A.H ? A.q : A.k;
-  const int h = head < A.H ? head : head - A.H;
+__device__ __forceinline__ void rotate_unit(const Args& A, unsigned token, unsigned b, unsigned t, unsigned head, unsigned u) {
+  const bool first = head < (unsigned)A.H;
+  const Side& s = first ? A.q : A.k;
+  const int h = first ? head : head - A.H;
   const T* x = static_cast<const T*>(s.x) + b * s.sb + t * s.st + h * s.sh;
   T* y = static_cast<T*>(s.y) + b * s.ob + t * s.ot + h * s.oh;
-  if (u >= turned) {  // copied
-    if (x == y) return;
-    float v[2 * PP];
-    ops::load(x + u * 2 * PP, v);
-    ops::store(y + u * 2 * PP, v);
-    return;
-  }
-  const long long p = !A.pos ? t : A.pos64 ? static_cast<const long long*>(A.pos)[bt] : static_cast<const int*>(A.pos)[bt];
+  const unsigned turned = A.R / (2 * PP);
+  const bool turn = u < turned;
+  if (!turn && x == y) return;
   float c[PP], sn[PP];
-  if (p >= 0 && p < A.positions) {
-    const float* row = A.table + p * A.R + u * PP;
-    ops::load(row, c);
-    ops::load(row + A.R / 2, sn);
-  } else {
+  if (turn) {
+    const long long p = !A.pos ? t : A.pos64 ? static_cast<const long long*>(A.pos)[token] : static_cast<const int*>(A.pos)[token];
+    if (p >= 0 && p < A.positions) {
+      const float* row = A.table + p * A.R + u * PP;
+      ops::load(row, c);
+      ops::load(row + A.R / 2, sn);
+    } else {
 #pragma unroll
-    for (int e = 0; e < PP; e++) c[e] = sn[e] = __builtin_nanf("");
+      for (int e = 0; e < PP; e++) c[e] = sn[e] = __builtin_nanf("");
+    }
+    if (A.inverse)
+#pragma unroll
+      for (int e = 0; e < PP; e++) sn[e] = -sn[e];
   }
-  const float sign = A.inverse ? -1.f : 1.f;
   if constexpr (INTERLEAVED) {
-    float v[2 * PP], w[2 * PP];
-    ops::load(x + u * 2 * PP, v);
+    float z[2 * PP];
+    ops::load(x + 2 * PP * u, z);
+    if (turn)
 #pragma unroll
-    for (int e = 0; e < PP; e++) {
-      w[2 * e] = v[2 * e] * c[e] - v[2 * e + 1] * (sign * sn[e]);
-      w[2 * e + 1] = v[2 * e + 1] * c[e] + v[2 * e] * (sign * sn[e]);
-    }
-    ops::store(y + u * 2 * PP, w);
+      for (int e = 0; e < PP; e++) {
+        const float a = z[2 * e], d = z[2 * e + 1];
+        z[2 * e] = a * c[e] - d * sn[e];
+        z[2 * e + 1] = d * c[e] + a * sn[e];
+      }
+    ops::store(y + 2 * PP * u, z);
   } else {
-    float v[PP], w[PP], a[PP], z[PP];
-    ops::load(x + u * PP, v);
-    ops::load(x + A.R / 2 + u * PP, w);
+    // the copied channels too in two halves
+    const unsigned lo = turn ? PP * u : A.R + PP * (u - turned), hi = lo + (turn ? A.R : A.D - A.R) / 2;
+    float v[PP], w[PP];
+    ops::load(x + lo, v);
+    ops::load(x + hi, w);
+    if (turn)
 #pragma unroll
-    for (int e = 0; e < PP; e++) {
-      a[e] = v[e] * c[e] - w[e] * (sign * sn[e]);
-      z[e] = w[e] * c[e] + v[e] * (sign * sn[e]);
-    }
-    ops::store(y + u * PP, a);
-    ops::store(y + A.R / 2 + u * PP, z);
+      for (int e = 0; e < PP; e++) {
+        const float a = v[e], d = w[e];
+        v[e] = a * c[e] - d * sn[e];
+        w[e] = d * c[e] + a * sn[e];
+      }
+    ops::store(y + lo, v);
+    ops::store(y + hi, w);
+  }
+}
+
+template <class T, int PP, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_kernel(Args A) {
+  const unsigned token0 = blockIdx.x * A.wg_tokens, items = min(A.wg_tokens, A.tokens - token0) * A.per;
+  for (unsigned i = threadIdx.x; i < items; i += 256) {
+    const unsigned k = divide(i, A.per, A.by_per), r = i - k * A.per, head = divide(r, A.units, A.by_units);
+    const unsigned token = token0 + k, b = A.T == A.tokens ? 0 : token / A.T;
+    rotate_unit<T, PP, INTERLEAVED>(A, token, b, token - b * A.T, head, r - head * A.units);
   }
 }
 

@@ -162,16 +162,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_gpu(
   Attention a = attention_of(q, k, v, log_decay, scale, state, lengths, false);
   const int64_t B = a.p.B, T = a.p.T, H = a.p.H, Hk = a.p.Hk, Dk = a.p.Dk, Dv = a.p.Dv;
   Tensor dq = at::empty({B, T, H, Dk}, q.options()), dk = at::empty({B, T, Hk, Dk}, q.options());
-  Tensor dv = at::empty({B, T, Hk, Dv}, q.options()), ds0 = at::empty({B, H, Dk, Dv}, q.options().dtype(at::kFloat));
+  Tensor dv = at::empty({B, T, Hk, Dv}, q.options());
+  // no gradient of a state that there is not
+  Tensor ds0 = a.state ? at::empty({B, H, Dk, Dv}, q.options().dtype(at::kFloat)) : at::empty({0}, q.options().dtype(at::kFloat));
   if (ds_in) {
     check_f32(LA, "the final state's gradient", *ds_in, q);
-    TORCH_CHECK(ds_in->sizes() == ds0.sizes(), LA, ": the final state's gradient must be ", ds0.sizes(), ", got ",
-                ds_in->sizes());
+    TORCH_CHECK(ds_in->sizes() == at::IntArrayRef({B, H, Dk, Dv}), LA,
+                ": the final state's gradient must be [B, H, Dk, Dv], got ", ds_in->sizes());
   }
   const OptTensor ds = dense(ds_in);
   if (B == 0 || H == 0) return {dq, dk, dv, ds0};
   if (T == 0) {
-    if (ds) ds0.copy_(*ds);
+    if (a.state && ds) ds0.copy_(*ds);
     else ds0.zero_();
     return {dq, dk, dv, ds0};
   }
@@ -185,7 +187,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_gpu(
   Tensor work = workspace(wb, q);
   check(sffft_linattn_bwd(&a.p, ptr(a.q), ptr(a.k), ptr(a.v), a.decay.const_data_ptr<float>(), cfptr(a.state),
                           a.lengths ? a.lengths->const_data_ptr<int>() : nullptr, ptr(go), cfptr(ds), dq.data_ptr(),
-                          dk.data_ptr(), dv.data_ptr(), fptr(ds0), wb ? work.data_ptr() : nullptr, wb, stream_of()),
+                          dk.data_ptr(), dv.data_ptr(), a.state ? fptr(ds0) : nullptr, wb ? work.data_ptr() : nullptr, wb, stream_of()),
         LA);
   return {dq, dk, dv, ds0};
 }
@@ -226,7 +228,8 @@ void rotary_run(const Tensor& q, const Tensor& k, const Tensor& table_in, const 
               ROT, ": table must be [positions, R] with R even and at most D = ", q.size(3), " (even too), got ",
               table_in.sizes());
   TORCH_CHECK(B <= INT32_MAX && T <= INT32_MAX && q.size(2) <= INT32_MAX && k.size(2) <= INT32_MAX &&
-                  q.size(3) <= INT32_MAX && table_in.size(0) <= INT32_MAX,
+                  q.size(3) <= INT32_MAX && table_in.size(0) <= INT32_MAX && B * T <= INT32_MAX &&
+                  (q.size(2) + k.size(2)) * (q.size(3) / 2) <= 65535,
               ROT, ": shape too large");
   OptTensor pos = dense(positions);
   if (pos) {
@@ -429,6 +432,12 @@ using NormBackwardSig = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tenso
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 Tensor plain(const OptTensor& t) { return t ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wants_grad(const OptTensor& t) { return t && wants_grad(*t); }
+// Whether a call is recorded: a node of the graph costs the host a microsecond or two, as much as a small kernel.
+template <class... A>
+bool recorded(const A&... t) {
+  return at::GradMode::is_enabled() && (wants_grad(t) || ...);
+}
 
 void refuse_second_derivative(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, " has no second derivative (backward with create_graph)");
@@ -465,6 +474,11 @@ std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& k, 
                                               const OptTensor& lengths) {
   TORCH_CHECK(!log_decay.requires_grad() || !at::GradMode::is_enabled(), LA,
               ": log_decay has no gradient (the decays are constants of the layer)");
+  if (!recorded(q, k, v, state)) {
+    static const auto op = op_handle<AttentionSig>("sffft::linear_attention");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(q, k, v, log_decay, scale, state, lengths);
+  }
   auto out = AttentionFn::apply(q, k, v, log_decay, scale, state, lengths);
   return {out[0], out[1]};
 }
@@ -472,8 +486,7 @@ std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& k, 
 Tensor step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state,
                      double scale, const OptTensor& slots) {
   static const auto op = op_handle<StepSig>("sffft::linear_attention_step");
-  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(state) ||
-                                               wants_grad(log_decay)),
+  TORCH_CHECK(!recorded(q, k, v, state, log_decay),
               "sffft::linear_attention_step has no gradient: use sffft::linear_attention");
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor o = op.call(q, k, v, log_decay, state, scale, slots);
@@ -509,6 +522,11 @@ class RotaryFn : public torch::autograd::Function<RotaryFn> {
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& table,
                                            const OptTensor& positions, bool interleaved, bool inverse) {
   TORCH_CHECK(!table.requires_grad() || !at::GradMode::is_enabled(), ROT, ": the table has no gradient");
+  if (!recorded(q, k)) {
+    static const auto op = op_handle<RotarySig>("sffft::rotary");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(q, k, table, positions, interleaved, inverse);
+  }
   auto out = RotaryFn::apply(q, k, table, positions, interleaved, inverse);
   return {out[0], out[1]};
 }
@@ -516,7 +534,7 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, con
 void rotary_inplace_autograd(const Tensor& q, const Tensor& k, const Tensor& table, const OptTensor& positions,
                              bool interleaved) {
   static const auto op = op_handle<RotaryInplaceSig>("sffft::rotary_");
-  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(q) || wants_grad(k)),
+  TORCH_CHECK(!recorded(q, k),
               "sffft::rotary_ records no gradient: use sffft::rotary");
   at::AutoDispatchBelowADInplaceOrView guard;
   op.call(q, k, table, positions, interleaved);
@@ -557,6 +575,11 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
 std::tuple<Tensor, Tensor> block_norm_autograd(const Tensor& x, const Tensor& y, const Tensor& w_pre,
                                                const OptTensor& w_post, const OptTensor& gate, const OptTensor& scale,
                                                c10::string_view activation, double eps) {
+  if (!recorded(x, y, w_pre, w_post, gate, scale)) {
+    static const auto op = op_handle<BlockNormSig>("sffft::block_norm");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(x, y, w_pre, w_post, gate, scale, activation, eps);
+  }
   auto out = BlockNormFn::apply(x, y, w_pre, w_post, gate, scale, activation, eps);
   return {out[0], out[1]};
 }
@@ -580,7 +603,14 @@ class PreNormFn : public torch::autograd::Function<PreNormFn> {
   }
 };
 
-Tensor pre_norm_autograd(const Tensor& x, const Tensor& w, double eps) { return PreNormFn::apply(x, w, eps); }
+Tensor pre_norm_autograd(const Tensor& x, const Tensor& w, double eps) {
+  if (!recorded(x, w)) {
+    static const auto op = op_handle<PreNormSig>("sffft::pre_norm");
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(x, w, eps);
+  }
+  return PreNormFn::apply(x, w, eps);
+}
 
 }  // namespace
 

@@ -110,7 +110,7 @@ def _linear_attention_fake(q, k, v, log_decay, scale, initial_state=None, length
 def _linear_attention_backward_fake(q, k, v, log_decay, scale, initial_state, lengths, grad_o, grad_state):
     B, T, H, Dk = q.shape
     return (q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape),
-            q.new_empty((B, H, Dk, v.shape[3]), dtype=torch.float32))
+            q.new_empty((0,) if initial_state is None else (B, H, Dk, v.shape[3]), dtype=torch.float32))
 
 
 @torch.library.register_fake("sffft::linear_attention_step")
