@@ -79,7 +79,7 @@ struct Reduce {
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int i = 0; i < N; i++) s.v[turn][i][w] = v[i];
-    __syncthreads();
+    ops::barrier();
 #pragma unroll
     for (int i = 0; i < N; i++) {
       v[i] = 0.f;
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(1024) void sum_kernel(SumArgs A) {
     for (; i < n; i += 32) s += p[i * A.C];
   }
   lds[g][lc] = s;
-  __syncthreads();
+  ops::barrier();
   // 32 lanes add 32 rows: lane (g, lc) of the first wavefronts takes column g
   s = lds[lc][g];
 #pragma unroll

@@ -190,6 +190,13 @@ struct Tile {
   }
 };
 
+// A 16-byte store. Its whole offset is the lane's: with a scalar register for a part of it the compiler leaves out the
+// wait between the store and the next write to its data registers, and where workgroups shared a CU the
+// store then sent what was written after it.
+__device__ __forceinline__ void store16(i32x4 x, __amdgpu_buffer_rsrc_t r, uint32_t at) {
+  __builtin_amdgcn_raw_buffer_store_b128(x, r, at, 0, 0);
+}
+
 // A chunk's rows of one operand on their way from memory to LDS: 16 bytes a piece, rows from n on and channels
 // from D on are zero and not read: their lanes' offsets lie beyond the buffer's records. One lane offset serves
 // every piece, the rest is in scalar registers.
@@ -388,7 +395,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
 #pragma unroll
       for (int i = 0; i < G::N; i++) {
         const i32x4 x = *reinterpret_cast<const i32x4*>(&ta.v[0][row + i * G::ROWS][col]);
-        __builtin_amdgcn_raw_buffer_store_b128(x, r, row + i * G::ROWS < left ? at : 0x80000000u, i * G::ROWS * orow * E, 0);
+        store16(x, r, row + i * G::ROWS < left ? at + i * G::ROWS * orow * E : 0x80000000u);
       }
     } else {
       const auto r = __builtin_amdgcn_make_buffer_rsrc(po, 0, 0x7fffffff, 0x00027000);
@@ -404,7 +411,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
             const i32x2 x = {(int)ops::pack_bf16(o[t][v][0], o[t][v][1]), (int)ops::pack_bf16(o[t][v][2], o[t][v][3])};
             __builtin_amdgcn_raw_buffer_store_b64(x, r, to, off, 0);
           } else {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, o[t][v]), r, to, off, 0);
+            store16(__builtin_bit_cast(i32x4, o[t][v]), r, in ? to + off : to);
           }
         }
     }
@@ -413,7 +420,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   float gn = 1.f;
   int have = -1;
   for (int c = 0; c < chunks; c++) {
-    __syncthreads();
+    ops::barrier();
     if constexpr (OUT) {  // the last chunk's
       store_out();
       if (c) po += (long long)dir * orow;
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
     t0 += dir;
     n = c + 1 < chunks ? count(t0) : 0;  // past the last chunk nothing is valid, and nothing is read
     fetch(n);
-    __syncthreads();
+    ops::barrier();
 
     if constexpr (OUT) {
       // P^T tiles: rows j, columns i
@@ -486,7 +493,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
 #pragma unroll
         for (int v = 0; v < VW; v++) o[t][v] *= f;
       }
-      __syncthreads();
+      ops::barrier();
     }
 
 #pragma unroll
@@ -532,7 +539,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
     if constexpr (OUT) stage_out();
   }
   if constexpr (OUT) {
-    if constexpr (VIA) __syncthreads();
+    if constexpr (VIA) ops::barrier();
     store_out();
   }
 
@@ -641,7 +648,7 @@ __global__ __launch_bounds__(256) void step_kernel(Operand q, Operand k, Operand
 #pragma unroll
     for (int e = 0; e < 4; e++) part[threadIdx.x >> 6][lc + e] = acc[e];
   }
-  __syncthreads();
+  ops::barrier();
   if (threadIdx.x < 16 && in) {
     float y[4];
 #pragma unroll

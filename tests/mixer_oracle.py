@@ -50,6 +50,32 @@ def attention_grads(q, k, v, log_decay, scale, go, gs, state=None, lengths=None)
     return (o.detach(), last.detach(), *grads)
 
 
+def attention_pairs(q, k, v, log_decay, scale, go, state, gs):
+    """(o, final, dq, dk, dv, d state) in 64 bits from every pair of tokens, on the inputs' device: for lengths
+    where the recurrence takes too long."""
+    B, T, H, Dk = q.shape
+    G = H // k.shape[2]
+    d = [x.detach().double() for x in (q, k, v, go)]
+    t = torch.arange(T, dtype=torch.float64, device=q.device)
+    out = [torch.zeros(s, dtype=torch.float64, device=q.device) for s in (go.shape, gs.shape, q.shape, k.shape, v.shape, gs.shape)]
+    gap = t[:, None] - t[None, :]
+    for b in range(B):
+        for h in range(H):
+            ld, hk = log_decay[h].double(), h // G
+            w = torch.where(gap >= 0, torch.exp(ld * gap.clamp(min=0)), torch.zeros_like(gap)) * scale
+            qh, kh, vh, oh = d[0][b, :, h], d[1][b, :, hk], d[2][b, :, hk], d[3][b, :, h]
+            s0, g1 = state[b, h].double(), gs[b, h].double()
+            since, left = torch.exp(ld * (t + 1))[:, None], torch.exp(ld * (T - 1 - t))[:, None]
+            p, r = (qh @ kh.t()) * w, (oh @ vh.t()) * w
+            out[0][b, :, h] = p @ vh + scale * since * (qh @ s0)
+            out[1][b, h] = (left * kh).t() @ vh + torch.exp(ld * T) * s0
+            out[2][b, :, h] = r @ kh + scale * since * (oh @ s0.t())
+            out[3][b, :, hk] += r.t() @ qh + left * (vh @ g1.t())
+            out[4][b, :, hk] += p.t() @ oh + left * (kh @ g1)
+            out[5][b, h] = scale * (since * qh).t() @ oh + torch.exp(ld * T) * g1
+    return out
+
+
 def rotary(x, table, positions, interleaved, inverse=False):
     """x [B, T, H, D] turned pair by pair; table [P, R] = cos | sin, positions [B, T] or None."""
     B, T, H, D = x.shape

@@ -62,6 +62,31 @@ def test_forward_and_gradients(dev, case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,H,Hk,Dk,Dv", [(3, 2001, 12, 12, 64, 64), (3, 2047, 12, 12, 128, 128), (2, 2500, 12, 12, 128, 64),
+                                            (2, 2500, 12, 4, 64, 128), (3, 2047, 12, 1, 96, 96)])
+def test_full_chip(dev, B, T, H, Hk, Dk, Dv, dtype):
+    """More workgroups than the chip has CUs, so that several share one, for every size of the tiles: no element off
+    by more than its row's size allows, and the same bits each time. (Stores of a workgroup that shared its CU once
+    sent registers that were overwritten behind them, and a barrier once let outputs be read from LDS too early.)"""
+    q, k, v, ld, s0, go, gs = inputs(dev, B, T, H, Hk, Dk, Dv, dtype, seed=T)
+    scale = Dk ** -0.5
+    want = mo.attention_pairs(q, k, v, ld, scale, go, s0, gs)
+    for t in (q, k, v, s0):
+        t.requires_grad_(True)
+    first = None
+    for _ in range(8):
+        o, s = torch.ops.sffft.linear_attention(q, k, v, ld, scale, s0)
+        got = (o, s, *torch.autograd.grad((o, s), (q, k, v, s0), (go, gs)))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+        for name, a, w in zip(("o", "state", "dq", "dk", "dv", "dstate"), got, want):
+            a = a.detach().double()
+            assert float((a - w).norm() / w.norm()) < (BF16 if got[0].dtype == torch.bfloat16 and name not in ("state", "dstate") else FP32), name
+            # the largest single error: 2^-6 (bf16) or 1e-4 of the largest value
+            assert float((a - w).abs().max()) < (2.0 ** -6 if dtype == torch.bfloat16 else 1e-4) * float(w.abs().max()), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("T,lengths", [(5, [0, 5, 1]), (130, [64, 0, 130]), (200, [199, 65, 63]), (64, [0, 0, 0])], ids=str)
 def test_lengths_and_what_lies_beyond_them(dev, T, lengths, dtype):
     """Tokens from lengths[b] on hold NaN and infinities: nothing of them reaches an output, their own are 0."""
