@@ -50,11 +50,14 @@ Cut cut_of(const sffft_linattn* p, int marches) {
   return {(chunks + per - 1) / per, per * C};
 }
 
+// Marches of the gradients' smallest launch (see backward): they share one where sizes and types are equal.
+int backward_marches(const sffft_linattn* p) { return p->Dk == p->Dv && (p->H == p->Hk || !p->io) ? 3 : 1; }
+
 template <class T, class TO, int KT, int VT, bool OUT, int UP>
 hipError_t launch(la::Launch& L, hipStream_t st) {
   L.vtiles = 1;
   for (int i = 0; i < L.nm; i++) L.vtiles = std::max(L.vtiles, (L.m[i].V + VT - 1) / VT);
-  const int units = L.s.B * L.s.H * (OUT ? L.nseg : L.nseg - 1);
+  const int units = L.s.B * L.s.H * (OUT || L.all ? L.nseg : L.nseg - 1);
   hipLaunchKernelGGL((la::march_kernel<T, TO, KT, VT, OUT, UP>), dim3((unsigned)((units + 7) / 8 * 8 * L.nm * L.vtiles)),
                      dim3(256), 0, st, L);
   return hipGetLastError();
@@ -72,7 +75,7 @@ hipError_t march_planes(la::Launch& L, hipStream_t st) {
 template <class T, bool OUT, class TO = T>
 hipError_t march(la::Launch L, hipStream_t st) {
   bool state = !OUT || sizeof(T) == 4;  // whether states leave in fp32
-  for (int i = 0; i < L.nm; i++) state = state || L.m[i].s1;
+  for (int i = 0; i < L.nm; i++) state = state || (L.m[i].s1 && !L.all);
   if constexpr (OUT && sizeof(T) == 2)
     if (!state) return march_planes<T, TO, OUT, 2>(L, st);
   return march_planes<T, TO, OUT, 3>(L, st);
@@ -96,6 +99,9 @@ size_t state_bytes(const sffft_linattn* p, const Cut& c) {
 }
 // More segments than this are joined by a launch of its own, fewer by each workgroup that follows them.
 constexpr int MAX_JOINED = 8;
+// From this many segments on the sum of the last one is made too, for the last state: it costs one more of many sums, and the
+// march then adds to its state only what outputs of 16 bits need.
+constexpr int MIN_ALL = 4;
 // dk and dv of heads that are shared, for each query head, before their sum
 size_t shared_bytes(const sffft_linattn* p) {
   return p->H == p->Hk ? 0 : (size_t)p->B * p->T * p->H * (p->Dk + p->Dv) * 4;
@@ -108,10 +114,14 @@ hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const v
   const Cut cut = cut_of(p, 1);
   const March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, work, s1, p->Dk, p->Dv, p->Dv, 1,
                    0, p->scale, p->scale, 1.f};
-  const la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1, cut.nseg > MAX_JOINED};
+  la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1, cut.nseg > MAX_JOINED,
+                  cut.nseg > MAX_JOINED || (s1 && cut.nseg >= MIN_ALL)};
   hipError_t e = hipSuccess;
   if (cut.nseg > 1) e = march<T, false>(L, st);
-  if (e == hipSuccess && L.scanned) e = scan({{{work, s0, p->Dk * p->Dv, 0}}, s, cut.nseg, cut.seg}, 1, st);
+  if (e == hipSuccess && L.scanned) {
+    e = scan({{{work, s0, s1, p->Dk * p->Dv, 0}}, s, cut.nseg, cut.seg}, 1, st);
+    L.m[0].s1 = nullptr;
+  }
   return e == hipSuccess ? march<T, true>(L, st) : e;
 }
 
@@ -122,18 +132,19 @@ hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const 
   const int G = p->H / p->Hk, Dk = p->Dk, Dv = p->Dv;
   const Operand Q = operand(q, p->q, 1), K = operand(k, p->k, G), V = operand(v, p->v, G), O = operand(go, p->go, 1);
   const size_t rows = (size_t)p->B * p->T;
-  const Cut cut = cut_of(p, 3);
+  const Cut cut = cut_of(p, backward_marches(p));
   const size_t states = state_bytes(p, cut) / 4;
   float *ws = work, *wd = ws + states, *wk = wd + states, *wv = wk + rows * p->H * Dk;
   const float c = p->scale;
-  const March mv = {K, Q, O, G > 1 ? wv : dv, ds1, wd, ds0, Dk, Dv, Dv, 1, 1, c, 1.f, c};
+  March mv = {K, Q, O, G > 1 ? wv : dv, ds1, wd, ds0, Dk, Dv, Dv, 1, 1, c, 1.f, c};
   la::Launch L = {{{Q, K, V, nullptr, s0, ws, nullptr, Dk, Dv, Dv, 1, 0, c, c, 1.f}, mv}, s, 2, cut.nseg, cut.seg, 1,
-                  cut.nseg > MAX_JOINED};
+                  cut.nseg > MAX_JOINED, cut.nseg > MAX_JOINED || (ds0 && cut.nseg >= MIN_ALL)};
   hipError_t e = hipSuccess;
   if (cut.nseg > 1) e = march<T, false>(L, st);
   if (e == hipSuccess && L.scanned)
-    e = scan({{{ws, s0, Dk * Dv, 0}, {wd, ds1, Dk * Dv, 1}}, s, cut.nseg, cut.seg}, 2, st);
+    e = scan({{{ws, s0, nullptr, Dk * Dv, 0}, {wd, ds1, ds0, Dk * Dv, 1}}, s, cut.nseg, cut.seg}, 2, st);
   if (e != hipSuccess) return e;
+  if (L.scanned) mv.s1 = nullptr;
   const March mq = {O, V, K, dq, s0, ws, nullptr, Dv, Dk, 1, Dv, 0, c, c, 1.f};
   const March mk = {V, O, Q, G > 1 ? wk : dk, ds1, wd, nullptr, Dv, Dk, 1, Dv, 1, c, 1.f, c};
   // One launch where the sizes and the types of the outputs are equal: what is summed afterwards leaves in fp32.
@@ -165,7 +176,7 @@ extern "C" {
 
 size_t sffft_linattn_work_bytes(const sffft_linattn* p, int backward) {
   if (!valid_shape(p)) return 0;
-  return backward ? 2 * state_bytes(p, cut_of(p, 3)) + shared_bytes(p) : state_bytes(p, cut_of(p, 1));
+  return backward ? 2 * state_bytes(p, cut_of(p, backward_marches(p))) + shared_bytes(p) : state_bytes(p, cut_of(p, 1));
 }
 
 int sffft_linattn_fwd(const sffft_linattn* p, const void* q, const void* k, const void* v, const float* log_decay,

@@ -61,12 +61,13 @@ struct Shape {
   const int* lengths;
 };
 
-// A launch: nm marches over B * H heads, nseg segments of seg tokens, vtiles tiles of the V channels. The sums are
-// made of all segments but the last of a march (the first if reversed).
+// A launch: nm marches over B * H heads, nseg segments of seg tokens, vtiles tiles of the V channels. Sums are made of
+// all segments, or of all but the last of a march (the first if reversed), whose sum nobody enters with: its
+// own workgroups then leave the last state.
 struct Launch {
   March m[3];
   Shape s;
-  int nm, nseg, seg, vtiles, scanned;
+  int nm, nseg, seg, vtiles, scanned, all;
 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -258,12 +259,12 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   // operands, follow each other on one of them.
   const int per = L.nm * L.vtiles, y = blockIdx.x >> 3;
   const int unit = y / per * 8 + (blockIdx.x & 7), sub = y % per;
-  const int segments = OUT ? L.nseg : L.nseg - 1;
+  const int segments = OUT || L.all ? L.nseg : L.nseg - 1;
   if (unit >= L.s.B * L.s.H * segments) return;
   const March m = L.m[sub / L.vtiles];
   const int v0 = sub % L.vtiles * VT;
   if (v0 >= m.V) return;
-  const int h = unit % L.s.H, zb = unit / L.s.H, b = zb / segments, z = zb % segments + (!OUT && m.rev);
+  const int h = unit % L.s.H, zb = unit / L.s.H, b = zb / segments, z = zb % segments + (!OUT && !L.all && m.rev);
   const long long bh = (long long)b * L.s.H + h;
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -340,11 +341,11 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
         for (int e = 0; e < 4; e++) x[a][v][e] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, off + e * m.sk * 4, 0));
       });
   };
-  auto store_state = [&](float* p) {
+  auto store_state = [&](float* p, const f32x4(&x)[KA][VW]) {
     const auto r = __builtin_amdgcn_make_buffer_rsrc(p, 0, 0x7fffffff, 0x00027000);
     state_tiles([&](int a, int v, uint32_t at, int off) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(S[a][v][e]), r, at, off + e * m.sk * 4, 0);
+      for (int e = 0; e < 4; e++) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(x[a][v][e]), r, at, off + e * m.sk * 4, 0);
     });
   };
 #pragma unroll
@@ -358,14 +359,20 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
     } else {
       if (m.s0) load_state(m.s0 + bh * kv, S);
       const int total = valid_tokens(L.s, b);
-      for (int y = rev ? L.nseg - 1 : 0; y != z; y += rev ? -1 : 1) {
+      auto join = [&](int y, f32x4(&x)[KA][VW]) {
         f32x4 u[KA][VW];
         load_state(sums + (long long)y * kv, u);
         const float d = power(min(max(total - y * L.seg, 0), L.seg));
 #pragma unroll
         for (int a = 0; a < KA; a++)
 #pragma unroll
-          for (int v = 0; v < VW; v++) S[a][v] = S[a][v] * d + u[a][v];
+          for (int v = 0; v < VW; v++) x[a][v] = S[a][v] * d + u[a][v];
+      };
+      for (int y = rev ? L.nseg - 1 : 0; y != z; y += rev ? -1 : 1) join(y, S);
+      if (L.all && m.s1 && z == (rev ? 0 : L.nseg - 1)) {  // the last state
+        f32x4 x[KA][VW];
+        join(z, x);
+        store_state(m.s1 + bh * kv, x);
       }
     }
   }
@@ -543,8 +550,8 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
     store_out();
   }
 
-  if constexpr (!OUT) store_state(m.sums + (bh * L.nseg + z) * kv);
-  else if (m.s1 && z == (rev ? 0 : L.nseg - 1)) store_state(m.s1 + bh * kv);
+  if constexpr (!OUT) store_state(m.sums + (bh * L.nseg + z) * kv, S);
+  else if (!L.all && m.s1 && z == (rev ? 0 : L.nseg - 1)) store_state(m.s1 + bh * kv, S);
 }
 
 // The states that enter the segments, from the sums of those before them, in place. Lane: four elements. Sixteen
@@ -552,6 +559,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
 struct Scan {
   float* sums;  // [bh][nseg][n]
   const float* s0;
+  float* s1;  // the last state
   int n, rev;
 };
 struct ScanLaunch {
@@ -573,7 +581,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
     float u[AHEAD][4];
 #pragma unroll
     for (int i = 0; i < AHEAD; i++)
-      if (z0 + i < L.nseg - 1) ops::load(p + (long long)(c.rev ? L.nseg - 1 - z0 - i : z0 + i) * c.n, u[i]);
+      if (z0 + i < L.nseg) ops::load(p + (long long)(c.rev ? L.nseg - 1 - z0 - i : z0 + i) * c.n, u[i]);
 #pragma unroll
     for (int i = 0; i < AHEAD; i++)
       if (z0 + i < L.nseg) {
@@ -584,6 +592,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
         for (int k = 0; k < 4; k++) x[k] = x[k] * d + u[i][k];
       }
   }
+  if (c.s1) ops::store(c.s1 + (long long)bh * c.n + e, x);
 }
 
 // Sum over the query heads that share a key/value head: out [rows][Hk][D] from in [rows][H][D].
