@@ -11,7 +11,11 @@
 // A row lies in the registers of one workgroup, 8 channels to a lane (16 beyond 8192 channels): every array crosses
 // memory once. A workgroup takes a run of rows and reads the next one before it works on this one (up to 4096 channels);
 // sums over rows stay in registers until its end, and the parts it leaves are added by a second kernel in a
-// fixed order. Bound by memory.
+// fixed order. Bound by memory: 16384 x 4 rows of 1536 in bf16, gate for each token, 561 us forward and backward for 2.6 GB.
+//
+// Rows of an odd width start anywhere between 16-byte boundaries. A workgroup then takes rows that start at the same distance from one
+// (every 2nd, 4th or 8th) and reads them from the boundary before the row on: the vectors stay aligned and the
+// lane's channels the same in all its rows, so that the sums over rows stay in registers.
 #pragma once
 #include "opsio.hpp"
 
@@ -26,9 +30,21 @@ struct Args {
   void *dx, *dy, *dgate;  // backward; dgate only where each row has its own gate
   float* parts;           // [quantity][part][C]: dwq, t, and the gate's where rows share one
   long long rows, gate_rows, block_rows;  // block_rows: rows that may share a workgroup
-  int C, act, part_rows, parts_per_block;
+  // A workgroup's part: part_rows rows, each `step` after the one before; `step` of them interleave
+  int C, act, part_rows, step, parts_per_block;
   long long nparts;
   float eps;
+};
+
+// Rows first, first + step, .. below last of part `part`.
+struct Part {
+  long long first, last;
+  __device__ __forceinline__ Part(const Args& A, int part) {
+    const int block = part / A.parts_per_block, k = part - block * A.parts_per_block, group = k / A.step;
+    const long long span = (long long)A.part_rows * A.step, base = block * A.block_rows;
+    first = base + group * span + (k - group * A.step);
+    last = min(min(base + (group + 1) * span, base + A.block_rows), A.rows);
+  }
 };
 
 // act(g) and its derivative
@@ -89,162 +105,270 @@ struct Reduce {
   }
 };
 
-// A lane's N channels of a row, as they are in memory (bf16 two to a register, unless they come one by
-// one): vector e of VEC at (e * lanes + lane) * VEC.
-template <class T, int VEC, int N>
+// Where a lane's N channels lie: vector e of VEC at places (e * lanes + lane) * VEC. The row's channels are the places from
+// `lo` to `hi`: it starts lo elements after a 16-byte boundary. (SHIFT; else lo is 0, and VEC divides C.)
+template <int VEC, int N, bool SHIFT>
+struct Places {
+  int lo, hi;
+  __device__ __forceinline__ int at(int e) const { return (e * (int)blockDim.x + (int)threadIdx.x) * VEC; }
+  __device__ __forceinline__ bool holds(int place) const { return (!SHIFT || place >= lo) && place < hi; }
+  // vector e lies in the row with all its elements
+  __device__ __forceinline__ bool whole(int e) const { return !SHIFT || (at(e) >= lo && at(e) + VEC <= hi); }
+};
+
+// A lane's channels of a row, as they are in memory (bf16 two to a register, unless they come one by one).
+template <class T, int VEC, int N, bool SHIFT>
 struct Row {
   static constexpr int PER = VEC == 1 ? 1 : 4 / (int)sizeof(T), WORDS = VEC / PER;
+  typedef Places<VEC, N, SHIFT> P;
   uint32_t w[N / PER];
-  __device__ __forceinline__ void load(const void* base, long long row, long long stride, int C) {
-    const T* p = static_cast<const T*>(base) + row * stride;
+  static __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+  static __device__ __forceinline__ uint32_t bits(uint16_t x) { return x; }
+  // element by element: of any alignment, nothing outside the row is read
+  __device__ __forceinline__ void load_elements(const T* p, int e, const P& at) {
+#pragma unroll
+    for (int i = 0; i < VEC; i++)
+      if (at.holds(at.at(e) + i)) w[(e * VEC + i) / PER] |= bits(p[at.at(e) + i]) << (sizeof(T) == 4 ? 0 : PER == 1 ? 16 : 16 * (i & 1));
+  }
+  // `edge`: the array's first or last row. In the others a vector that is not whole is read as a whole, with elements of the
+  // neighbouring rows, which mask() clears.
+  __device__ __forceinline__ void load(const void* base, long long row, long long stride, const P& at, bool edge) {
+    const T* p = static_cast<const T*>(base) + row * stride - (SHIFT ? at.lo : 0);
 #pragma unroll
     for (int e = 0; e < N / VEC; e++) {
-      const int at = (e * (int)blockDim.x + (int)threadIdx.x) * VEC;
       uint32_t* d = w + e * WORDS;
 #pragma unroll
       for (int i = 0; i < WORDS; i++) d[i] = 0;
-      if (at < C) {
-        if constexpr (WORDS == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(p + at);
-          d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
-        } else if constexpr (WORDS == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(p + at);
-          d[0] = v.x, d[1] = v.y;
-        } else if constexpr (sizeof(T) == 4) {
-          d[0] = __float_as_uint(p[at]);
+      if (at.at(e) < at.hi) {
+        if constexpr (VEC == 1) {
+          load_elements(p, e, at);
+        } else if (SHIFT && edge && !at.whole(e)) {
+          load_elements(p, e, at);
         } else {
-          d[0] = (uint32_t)p[at] << 16;
+          if constexpr (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p + at.at(e));
+            d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(p + at.at(e));
+            d[0] = v.x, d[1] = v.y;
+          }
         }
       }
     }
+  }
+  __device__ __forceinline__ void load_any(const void* base, long long row, long long stride, const P& at) {
+    const T* p = static_cast<const T*>(base) + row * stride - (SHIFT ? at.lo : 0);
+#pragma unroll
+    for (int i = 0; i < N / PER; i++) w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < N / VEC; e++) load_elements(p, e, at);
+  }
+  __device__ __forceinline__ void mask(const uint32_t (&m)[N / PER]) {
+    if constexpr (SHIFT)
+#pragma unroll
+      for (int i = 0; i < N / PER; i++) w[i] &= m[i];
   }
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (PER == 2) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     else return __uint_as_float(w[i]);
   }
 };
-template <class T, int VEC, int N>
-__device__ __forceinline__ void put_row(void* base, long long row, int C, const float (&x)[N]) {
-  T* p = static_cast<T*>(base) + row * C;
+template <class T, int VEC, int N, bool SHIFT>
+__device__ __forceinline__ void put_row(void* base, long long row, int C, const Places<VEC, N, SHIFT>& at, const float (&x)[N]) {
+  T* p = static_cast<T*>(base) + row * C - (SHIFT ? at.lo : 0);
 #pragma unroll
   for (int e = 0; e < N / VEC; e++) {
-    const int at = (e * (int)blockDim.x + (int)threadIdx.x) * VEC;
-    float t[VEC];
+    if (SHIFT && !at.whole(e)) {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) t[i] = x[e * VEC + i];
-    if (at < C) ops::store(p + at, t);
+      for (int i = 0; i < VEC; i++)
+        if (at.holds(at.at(e) + i)) ops::put(p + at.at(e) + i, x[e * VEC + i]);
+    } else if (at.at(e) < at.hi) {
+      float t[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; i++) t[i] = x[e * VEC + i];
+      ops::store(p + at.at(e), t);
+    }
   }
 }
-// weights, 1 where there are none
-template <int VEC, int N>
-__device__ __forceinline__ void weights(const float* p, int C, float (&x)[N]) {
+// sums, channel by channel where the row is shifted: their rows are aligned in another way
+template <int VEC, int N, bool SHIFT>
+__device__ __forceinline__ void put_sums(float* base, long long part, int C, const Places<VEC, N, SHIFT>& at, const float (&x)[N]) {
+  if constexpr (!SHIFT) {
+    put_row<float>(base, part, C, at, x);
+  } else {
+    float* p = base + part * C - at.lo;
+#pragma unroll
+    for (int e = 0; e < N / VEC; e++)
+#pragma unroll
+      for (int i = 0; i < VEC; i++)
+        if (at.holds(at.at(e) + i)) p[at.at(e) + i] = x[e * VEC + i];
+  }
+}
+// weights, 1 where there are none; 0 outside the row
+template <int VEC, int N, bool SHIFT>
+__device__ __forceinline__ void weights(const float* p, const Places<VEC, N, SHIFT>& at, float (&x)[N]) {
 #pragma unroll
   for (int e = 0; e < N / VEC; e++) {
-    const int at = (e * (int)blockDim.x + (int)threadIdx.x) * VEC;
-    float t[VEC];
-    if (p && at < C) ops::load(p + at, t);
+    if constexpr (SHIFT) {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) x[e * VEC + i] = !p ? 1.f : at < C ? t[i] : 0.f;
+      for (int i = 0; i < VEC; i++) x[e * VEC + i] = !at.holds(at.at(e) + i) ? 0.f : p ? p[at.at(e) + i - at.lo] : 1.f;
+    } else {
+      float t[VEC];
+      const bool in = at.at(e) < at.hi;
+      if (p && in) ops::load(p + at.at(e), t);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) x[e * VEC + i] = !p ? 1.f : in ? t[i] : 0.f;
+    }
   }
 }
 
-template <class T, int VEC, int N, int BLK, bool Y>
+// What both kernels share: the lane's places, the mask of its elements, and the gates that rows share.
+template <class T, int VEC, int N, bool SHIFT>
+struct Lane {
+  typedef Row<T, VEC, N, SHIFT> R;
+  Places<VEC, N, SHIFT> at;
+  uint32_t m[N / R::PER];
+  __device__ __forceinline__ Lane(const Args& A, long long first) {
+    at.lo = 0;
+    if constexpr (SHIFT)
+      at.lo = (int)((reinterpret_cast<uintptr_t>(A.x) + (uintptr_t)(first * A.sx) * sizeof(T)) % 16 / sizeof(T));
+    at.hi = at.lo + A.C;
+    if constexpr (SHIFT)
+#pragma unroll
+      for (int i = 0; i < N / R::PER; i++) {
+        const int p = at.at(i / R::WORDS) + i % R::WORDS * R::PER;
+        m[i] = R::PER == 1 ? (at.holds(p) ? ~0u : 0u) : (at.holds(p) ? 0xffffu : 0u) | (at.holds(p + 1) ? 0xffff0000u : 0u);
+      }
+  }
+  // gate i, which lies at another distance from a boundary than the rows
+  __device__ __forceinline__ void gate(const Args& A, long long i, R& g) const {
+    if constexpr (SHIFT) g.load_any(A.gate, i, A.sg, at);
+    else g.load(A.gate, i, A.sg, at, false);
+  }
+};
+
+template <class T, int VEC, int N, int BLK, bool SHIFT, bool Y>
 __global__ __launch_bounds__(BLK) void fwd_kernel(Args A) {
   constexpr bool AHEAD = BLK <= 512;  // 1024 lanes leave each 128 registers: none for a row in advance
   __shared__ Sums sums;
   Reduce reduce = {sums, (int)blockDim.x >> 6, 0};
-  const long long first = (long long)blockIdx.x * A.part_rows, last = min(first + A.part_rows, A.rows);
+  const Part part(A, blockIdx.x);
+  Lane<T, VEC, N, SHIFT> lane(A, part.first);
+  const auto& at = lane.at;
+  const bool shared = A.gate && A.gate_rows > 1;
   float wq[N], ws[N];
-  weights<VEC>(A.wq, A.C, wq);
+  weights(A.wq, at, wq);
   if constexpr (Y) {
     float sc[N];
-    weights<VEC>(A.wp, A.C, ws);
-    weights<VEC>(A.sc, A.C, sc);
+    weights(A.wp, at, ws);
+    weights(A.sc, at, sc);
 #pragma unroll
     for (int i = 0; i < N; i++) ws[i] *= sc[i];
   }
   const float inv = 1.f / (float)A.C;
-  Row<T, VEC, N> nx, ny, ng;
+  Row<T, VEC, N, SHIFT> nx, ny, ng, rg;
   auto fetch = [&](long long row) {
-    nx.load(A.x, row, A.sx, A.C);
+    const bool edge = row == 0 || row == A.rows - 1;
+    nx.load(A.x, row, A.sx, at, edge);
     if constexpr (Y) {
-      ny.load(A.y, row, A.sy, A.C);
-      if (A.gate) ng.load(A.gate, A.gate_rows == 1 ? row : row / A.gate_rows, A.sg, A.C);
+      ny.load(A.y, row, A.sy, at, edge);
+      if (A.gate && !shared) ng.load(A.gate, row, A.sg, at, edge);
     }
   };
-  if (AHEAD) fetch(first);
-  for (long long row = first; row < last; row++) {
-    if (!AHEAD) fetch(row);
-    const Row<T, VEC, N> rx = nx, ry = ny, rg = ng;
-    if (AHEAD && row + 1 < last) fetch(row + 1);
-    float x[N], s[1];
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = rx[i];
-    if constexpr (Y) {
-      float f = 1.f, d;
-      if (A.wp) {
-        s[0] = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
-        reduce(s);
-        f = 1.f / sqrtf(s[0] * inv + A.eps);
+  if (AHEAD && part.first < part.last) fetch(part.first);
+  long long gate = shared ? part.first / A.gate_rows : 0;  // rows that share one are worked on together
+  for (long long row = part.first; row < part.last; gate++) {
+    long long stop = part.last;
+    if constexpr (Y)
+      if (shared) {
+        lane.gate(A, gate, rg);
+        stop = min(stop, (gate + 1) * A.gate_rows);
       }
-#pragma unroll
-      for (int i = 0; i < N; i++) {
-        float m = ry[i] * f * ws[i];
-        if (A.gate) m *= activate(A.act, rg[i], &d);
-        x[i] += m;
+    for (; row < stop; row += A.step) {
+      if (!AHEAD) fetch(row);
+      Row<T, VEC, N, SHIFT> rx = nx, ry = ny;
+      rx.mask(lane.m);
+      if constexpr (Y) {
+        ry.mask(lane.m);
+        if (!shared) rg = ng, rg.mask(lane.m);
       }
-      put_row<T, VEC>(A.r, row, A.C, x);
+      if (AHEAD && row + A.step < part.last) fetch(row + A.step);
+      float x[N], s[1];
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = rx[i];
+      if constexpr (Y) {
+        float f = 1.f, d;
+        if (A.wp) {
+          s[0] = 0.f;
+#pragma unroll
+          for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
+          reduce(s);
+          f = 1.f / sqrtf(s[0] * inv + A.eps);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          float m = ry[i] * f * ws[i];
+          if (A.gate) m *= activate(A.act, rg[i], &d);
+          x[i] += m;
+        }
+        put_row<T>(A.r, row, A.C, at, x);
+      }
+      s[0] = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; i++) s[0] += x[i] * x[i];
+      reduce(s);
+      const float f = 1.f / sqrtf(s[0] * inv + A.eps);
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] *= f * wq[i];
+      put_row<T>(A.h, row, A.C, at, x);
     }
-    s[0] = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; i++) s[0] += x[i] * x[i];
-    reduce(s);
-    const float f = 1.f / sqrtf(s[0] * inv + A.eps);
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] *= f * wq[i];
-    put_row<T, VEC>(A.h, row, A.C, x);
   }
 }
 
-template <class T, int VEC, int N, int BLK, bool Y>
+template <class T, int VEC, int N, int BLK, bool SHIFT, bool Y>
 __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
   constexpr bool AHEAD = BLK <= 512;  // 1024 lanes leave each 128 registers: none for a row in advance
   __shared__ Sums sums;
   Reduce reduce = {sums, (int)blockDim.x >> 6, 0};
-  const long long part = blockIdx.x, block = part / A.parts_per_block;
-  const long long first = block * A.block_rows + (part - block * A.parts_per_block) * A.part_rows;
-  const long long last = min(min(first + A.part_rows, (block + 1) * A.block_rows), A.rows);
+  const Part part(A, blockIdx.x);
+  Lane<T, VEC, N, SHIFT> lane(A, part.first);
+  const auto& at = lane.at;
   const bool shared = A.gate && A.gate_rows > 1;
   const float inv = 1.f / (float)A.C;
   float wq[N], wp[N], sc[N], dwq[N], t[N];
-  weights<VEC>(A.wq, A.C, wq);
+  weights(A.wq, at, wq);
 #pragma unroll
   for (int i = 0; i < N; i++) dwq[i] = t[i] = 0.f;
   if constexpr (Y) {
-    weights<VEC>(A.wp, A.C, wp);
-    weights<VEC>(A.sc, A.C, sc);
+    weights(A.wp, at, wp);
+    weights(A.sc, at, sc);
   }
-  Row<T, VEC, N> nx, ny, ng, nr, nh;
+  Row<T, VEC, N, SHIFT> nx, ny, ng, nr, nh;
   auto fetch = [&](long long row) {
-    nx.load(A.x, row, A.sx, A.C);
+    const bool edge = row == 0 || row == A.rows - 1;
+    nx.load(A.x, row, A.sx, at, edge);
     if constexpr (Y) {
-      ny.load(A.y, row, A.sy, A.C);
-      if (A.gate) ng.load(A.gate, shared ? row / A.gate_rows : row, A.sg, A.C);
+      ny.load(A.y, row, A.sy, at, edge);
+      if (A.gate && !shared) ng.load(A.gate, row, A.sg, at, edge);
     }
-    if (A.gr) nr.load(A.gr, row, A.sgr, A.C);
-    if (A.gh) nh.load(A.gh, row, A.sgh, A.C);
+    if (A.gr) nr.load(A.gr, row, A.sgr, at, edge);
+    if (A.gh) nh.load(A.gh, row, A.sgh, at, edge);
   };
   if (!A.gr) nr = {};
   if (!A.gh) nh = {};
-  if (AHEAD) fetch(first);
-  Row<T, VEC, N> rg = {};
-  for (long long row = first; row < last; row++) {
+  if (AHEAD && part.first < part.last) fetch(part.first);
+  Row<T, VEC, N, SHIFT> rg = {};
+  if constexpr (Y)  // rows of a part share theirs
+    if (shared && part.first < part.last) lane.gate(A, part.first / A.gate_rows, rg);
+  for (long long row = part.first; row < part.last; row += A.step) {
     if (!AHEAD) fetch(row);
-    const Row<T, VEC, N> rx = nx, ry = ny, rr = nr, rh = nh;
-    rg = ng;
-    if (AHEAD && row + 1 < last) fetch(row + 1);
+    Row<T, VEC, N, SHIFT> rx = nx, ry = ny, rr = nr, rh = nh;
+    rx.mask(lane.m), rr.mask(lane.m), rh.mask(lane.m);
+    if constexpr (Y) {
+      ry.mask(lane.m);
+      if (!shared) rg = ng, rg.mask(lane.m);
+    }
+    if (AHEAD && row + A.step < part.last) fetch(row + A.step);
     float r[N], y[N], act[N], s[1], fy = 1.f, d;
 #pragma unroll
     for (int i = 0; i < N; i++) r[i] = rx[i];
@@ -275,7 +399,7 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
       dwq[i] += rh[i] * r[i];
       dr[i] = rr[i] + fr * (rh[i] * wq[i] - r[i] * mean);
     }
-    put_row<T, VEC>(A.dx, row, A.C, dr);
+    put_row<T>(A.dx, row, A.C, at, dr);
     if constexpr (Y) {
       if (shared) {
 #pragma unroll
@@ -291,7 +415,7 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
           activate(A.act, rg[i], &d);
           g[i] = dr[i] * sc[i] * y[i] * wp[i] * d;
         }
-        put_row<T, VEC>(A.dgate, row, A.C, g);
+        put_row<T>(A.dgate, row, A.C, at, g);
       }
 #pragma unroll
       for (int i = 0; i < N; i++) dr[i] *= sc[i] * act[i];
@@ -307,10 +431,10 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
 #pragma unroll
         for (int i = 0; i < N; i++) dr[i] = fy * (dr[i] - y[i] * my);
       }
-      put_row<T, VEC>(A.dy, row, A.C, dr);
+      put_row<T>(A.dy, row, A.C, at, dr);
     }
   }
-  put_row<float, VEC>(A.parts, part, A.C, dwq);
+  put_sums(A.parts, blockIdx.x, A.C, at, dwq);
   if constexpr (Y) {
     if (shared) {
       float g[N], d;
@@ -320,9 +444,9 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
         g[i] = t[i] * sc[i] * wp[i] * d;
         t[i] *= a;
       }
-      put_row<float, VEC>(A.parts, 2 * A.nparts + part, A.C, g);
+      put_sums(A.parts, 2 * A.nparts + blockIdx.x, A.C, at, g);
     }
-    put_row<float, VEC>(A.parts, A.nparts + part, A.C, t);
+    put_sums(A.parts, A.nparts + blockIdx.x, A.C, at, t);
   }
 }
 

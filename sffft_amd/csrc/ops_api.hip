@@ -4,6 +4,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 
 #include "blocknorm.hpp"
 #include "ops_status.hpp"
@@ -49,62 +50,69 @@ hipError_t rotary(rot::Args a, bool interleaved, bool wide, hipStream_t st) {
 
 // ---- norms ----
 
-// How a row lies in registers: N channels to a lane, in loads of `vec`; the fewest wavefronts that hold it.
+// How a row is read: in vectors of 16 bytes; in vectors of 8 (bf16); of 16 from the boundary before the row on (SHIFTED); or channel by
+// channel.
+enum Access { WHOLE, HALVES, SHIFTED, SINGLE };
+// How it lies in registers: n channels to a lane, the fewest wavefronts that hold it. Rows that start at the same distance from a
+// boundary are `step` apart.
 struct RowShape {
-  int vec, n, waves;
+  Access access;
+  int n, waves, step;
 };
-RowShape row_shape(int C, int vec) {
-  const int n = C > 8192 ? 16 : 8;
-  return {vec, n, (C + 64 * n - 1) / (64 * n)};
+RowShape row_shape(const sffft_blocknorm* p, Access access) {
+  const int V = p->io ? 8 : 4, places = p->C + (access == SHIFTED ? V - 1 : 0), n = places > 8192 ? 16 : 8;
+  int step = 1;
+  while (access == SHIFTED && (long long)step * p->C % V) step *= 2;
+  return {access, n, (places + 64 * n - 1) / (64 * n), step};
 }
+constexpr int MAX_WAVES = 16;
 
-// Rows in parts that one workgroup each takes: about `fill` wavefronts for each of 256 CUs, no part across rows
-// of different gates.
+// Rows in parts that one workgroup each takes: as many workgroups as `fill` wavefronts on each of 256 CUs hold (one round of
+// them: a second one for a few more would double the time), no part across rows of different gates.
 struct Parts {
   long long block_rows, blocks, nparts;
-  int part_rows, per_block;
+  int part_rows, step, per_block;
 };
 Parts parts_of(const sffft_blocknorm* p, const RowShape& s, bool shared_gate, int fill) {
   Parts q;
   q.block_rows = shared_gate ? p->gate_rows : p->rows;
   q.blocks = p->rows / q.block_rows;
-  const long long want = std::max<long long>(1, 256 * fill / s.waves / q.blocks);
-  const long long per = std::min(want, q.block_rows);
-  q.part_rows = (int)std::min<long long>((q.block_rows + per - 1) / per, INT_MAX / 2);
-  q.per_block = (int)((q.block_rows + q.part_rows - 1) / q.part_rows);
+  q.step = (int)std::min<long long>(s.step, q.block_rows);
+  const long long groups = std::max<long long>(1, 256 * std::max(1, fill / s.waves) / q.blocks / q.step);
+  const long long run = (q.block_rows + q.step - 1) / q.step;  // rows of a class
+  q.part_rows = (int)std::min<long long>((run + groups - 1) / groups, INT_MAX / 16);
+  q.per_block = (int)std::min<long long>((run + q.part_rows - 1) / q.part_rows * q.step, INT_MAX);
   q.nparts = q.blocks * q.per_block;
   return q;
 }
 // Registers allow about 12 wavefronts for the backward kernel and 24 for the forward one.
 constexpr int FILL_FWD = 24, FILL_BWD = 12;
 
-template <class T, int VEC, int N, int BLK>
+template <class T, int VEC, int N, int BLK, bool SHIFT>
 void norm_launch(const bn::Args& a, int waves, bool y, bool backward, dim3 grid, hipStream_t st) {
   const dim3 block(64u * waves);
   if (backward) {
-    if (y) hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, N, BLK, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, N, BLK, false>), grid, block, 0, st, a);
+    if (y) hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, N, BLK, SHIFT, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((bn::bwd_kernel<T, VEC, N, BLK, SHIFT, false>), grid, block, 0, st, a);
   } else {
-    if (y) hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, N, BLK, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, N, BLK, false>), grid, block, 0, st, a);
+    if (y) hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, N, BLK, SHIFT, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((bn::fwd_kernel<T, VEC, N, BLK, SHIFT, false>), grid, block, 0, st, a);
   }
 }
-template <class T, int VEC>
-void norm_vec(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
-  if (s.n == 16) norm_launch<T, VEC, 16, 1024>(a, s.waves, y, backward, grid, st);
-  else if (s.waves > 8) norm_launch<T, VEC, 8, 1024>(a, s.waves, y, backward, grid, st);
-  else if (s.waves > 4) norm_launch<T, VEC, 8, 512>(a, s.waves, y, backward, grid, st);
-  else norm_launch<T, VEC, 8, 256>(a, s.waves, y, backward, grid, st);
+template <class T, int VEC, bool SHIFT = false>
+void norm_access(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
+  if (s.n == 16) norm_launch<T, VEC, 16, 1024, SHIFT>(a, s.waves, y, backward, grid, st);
+  else if (s.waves > 8) norm_launch<T, VEC, 8, 1024, SHIFT>(a, s.waves, y, backward, grid, st);
+  else if (s.waves > 4) norm_launch<T, VEC, 8, 512, SHIFT>(a, s.waves, y, backward, grid, st);
+  else norm_launch<T, VEC, 8, 256, SHIFT>(a, s.waves, y, backward, grid, st);
 }
 template <class T>
 hipError_t norm(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
-  if (s.vec == 8) {
-    if constexpr (sizeof(T) == 2) norm_vec<T, 8>(a, s, y, backward, grid, st);
-  } else if (s.vec == 4) {
-    norm_vec<T, 4>(a, s, y, backward, grid, st);
-  } else {
-    norm_vec<T, 1>(a, s, y, backward, grid, st);
-  }
+  constexpr int V = 16 / sizeof(T);
+  if (s.access == WHOLE) norm_access<T, V>(a, s, y, backward, grid, st);
+  else if (s.access == SHIFTED) norm_access<T, V, true>(a, s, y, backward, grid, st);
+  else if (s.access == SINGLE) norm_access<T, 1>(a, s, y, backward, grid, st);
+  else if constexpr (V == 8) norm_access<T, 4>(a, s, y, backward, grid, st);
   return hipGetLastError();
 }
 
@@ -138,17 +146,39 @@ bool apart(const Span* in, int ni, const Span* out, int no) {
   return true;
 }
 
-// The widest loads, of 16 bytes or of four channels, that every array's rows are aligned to; else one by one.
-int vector_of(const sffft_blocknorm* p, const Span* all, int n, const long long* strides, int ns, const float* const w[3]) {
-  const int elem = p->io ? 2 : 4;
-  for (int vec : {16 / elem, 4}) {
-    bool ok = p->C % vec == 0;
-    for (int i = 0; i < n; i++) ok = ok && ops::aligned(all[i].p, vec * elem);
-    for (int i = 0; i < ns; i++) ok = ok && strides[i] % vec == 0;
-    for (int i = 0; i < 3; i++) ok = ok && ops::aligned(w[i], 16);
-    if (ok) return vec;
-  }
-  return 1;
+// WHOLE (HALVES) where every row starts and ends at a boundary of 16 (8) bytes, SHIFTED where those of all arrays start at the same
+// distance from one of 16 (a gate that rows share is read seldom and does not count). A training step over 25 M elements with a gate
+// for each token, us: bf16 C = 1531 SINGLE 897, SHIFTED 223; 2047 903, 357; 5001 986, 338; fp32 1531 312, 303; 2047 343, 435; 5001
+// 468, 415; bf16 1028 HALVES 192, SHIFTED 248.
+struct RowArray {
+  const void* p;
+  long long stride;
+};
+Access access_of(const sffft_blocknorm* p, std::initializer_list<RowArray> arrays, RowArray gate, const float* const (&w)[3]) {
+  const int elem = p->io ? 2 : 4, V = 16 / elem;
+  int vec = p->C % V ? p->C % 4 ? 1 : 4 : V;  // what is aligned
+  // (a row of SHIFTED has 16 bytes at least: what is read beside it then lies in its neighbours)
+  bool shifted = p->C >= V;
+  const auto whole = [&](const RowArray& a) {
+    if (!a.p) return;
+    while (vec > 1 && (!ops::aligned(a.p, vec * elem) || a.stride % vec)) vec = vec > 4 ? 4 : 1;
+  };
+  const auto look = [&](const RowArray& a) {
+    if (!a.p) return;
+    whole(a);
+    shifted = shifted && ((uintptr_t)a.p - (uintptr_t)arrays.begin()->p) % 16 == 0 &&
+              (p->rows == 1 || (a.stride >= p->C && (a.stride - p->C) % V == 0));
+  };
+  for (const RowArray& a : arrays) look(a);
+  if (p->gate_rows == 1) look(gate);
+  else whole(gate);
+  for (const float* x : w)
+    if (!ops::aligned(x, 16)) vec = 1;
+  if (vec == V) return WHOLE;
+  if (vec == 4) return HALVES;
+  // fp32 rows that would take one more wavefront are faster channel by channel: two workgroups of 5 on a CU instead of three of 4
+  const int waves = row_shape(p, SHIFTED).waves;
+  return shifted && (p->io ? waves <= MAX_WAVES : waves == row_shape(p, SINGLE).waves) ? SHIFTED : SINGLE;
 }
 
 }  // namespace
@@ -238,16 +268,15 @@ int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, 
   for (int i = 0; i < 6; i++)
     if (!ops::aligned(in[i].p, i < 3 ? elem : 4)) return SFFFT_EINVAL;
   if (!ops::aligned(r, elem) || !ops::aligned(h, elem) || !apart(in, 6, out, 2)) return SFFFT_EINVAL;
-  const long long strides[] = {p->x, y ? p->y : 0, gate ? p->gate : 0};
-  const Span act[] = {{x, 0}, {y, 0}, {gate, 0}, {r, 0}, {h, 0}};
-  const float* const w[] = {w_pre, w_post, scale};
-  const RowShape s = row_shape(p->C, vector_of(p, act, 5, strides, 3, w));
+  const RowShape s = row_shape(p, access_of(p, {{x, p->x}, {y, p->y}, {r, p->C}, {h, p->C}}, {gate, p->gate},
+                                            {w_pre, w_post, scale}));
   const Parts q = parts_of(p, s, false, FILL_FWD);
   if (q.nparts > INT_MAX) return SFFFT_EINVAL;
   bn::Args a = {};
   a.x = x, a.y = y, a.gate = gate, a.sx = p->x, a.sy = p->y, a.sg = p->gate;
   a.wq = w_pre, a.wp = w_post, a.sc = scale, a.r = r, a.h = h;
-  a.rows = p->rows, a.gate_rows = p->gate_rows, a.C = p->C, a.act = p->act, a.eps = p->eps, a.part_rows = q.part_rows;
+  a.rows = p->rows, a.gate_rows = p->gate_rows, a.C = p->C, a.act = p->act, a.eps = p->eps;
+  a.block_rows = q.block_rows, a.part_rows = q.part_rows, a.step = q.step, a.parts_per_block = q.per_block;
   const auto run = p->io ? norm<uint16_t> : norm<float>;
   return ops::hip_status(run(a, s, y != nullptr, false, dim3((unsigned)q.nparts), (hipStream_t)stream),
                          "block norm launch");
@@ -256,8 +285,9 @@ int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, 
 size_t sffft_blocknorm_work_bytes(const sffft_blocknorm* p, int has_y, int has_gate) {
   if (!valid_norm(p)) return 0;
   const bool shared = has_gate && p->gate_rows > 1;
-  const Parts q = parts_of(p, row_shape(p->C, 1), shared, FILL_BWD);  // the width of the loads changes nothing in it
-  return (size_t)(has_y ? shared ? 3 : 2 : 1) * q.nparts * p->C * 4;
+  long long n = 0;  // of any access: where the arrays lie is not known yet
+  for (Access a : {WHOLE, SHIFTED}) n = std::max(n, parts_of(p, row_shape(p, a), shared, FILL_BWD).nparts);
+  return (size_t)(has_y ? shared ? 3 : 2 : 1) * n * p->C * 4;
 }
 
 int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, const void* gate, const float* w_pre,
@@ -284,10 +314,9 @@ int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, 
   for (int i = 0; i < 6; i++)
     if (!ops::aligned(out[i].p, i < 3 ? elem : 4)) return SFFFT_EINVAL;
   if (!apart(in, 8, out, 7)) return SFFFT_EINVAL;
-  const long long strides[] = {p->x, y ? p->y : 0, gate ? p->gate : 0, gr ? p->gr : 0, gh ? p->gh : 0};
-  const Span act[] = {{x, 0}, {y, 0}, {gate, 0}, {gr, 0}, {gh, 0}, {dx, 0}, {dy, 0}, {dgate, 0}};
-  const float* const w[] = {w_pre, w_post, scale};
-  const RowShape s = row_shape(p->C, vector_of(p, act, 8, strides, 5, w));
+  const RowArray gates_in = {gate, p->gate}, gates_out = {shared ? nullptr : dgate, p->C};
+  const RowShape s = row_shape(p, access_of(p, {{x, p->x}, {y, p->y}, {gr, p->gr}, {gh, p->gh}, {dx, p->C}, {dy, p->C}, gates_out},
+                                            gates_in, {w_pre, w_post, scale}));
   const Parts q = parts_of(p, s, shared, FILL_BWD);
   if (q.nparts > INT_MAX) return SFFFT_EINVAL;
   bn::Args a = {};
@@ -295,7 +324,7 @@ int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, 
   a.sx = p->x, a.sy = p->y, a.sg = p->gate, a.sgr = p->gr, a.sgh = p->gh;
   a.wq = w_pre, a.wp = w_post, a.sc = scale, a.dx = dx, a.dy = dy, a.dgate = dgate;
   a.parts = static_cast<float*>(work), a.rows = p->rows, a.gate_rows = gate ? p->gate_rows : 1;
-  a.block_rows = q.block_rows, a.C = p->C, a.act = p->act, a.part_rows = q.part_rows, a.parts_per_block = q.per_block;
+  a.block_rows = q.block_rows, a.C = p->C, a.act = p->act, a.part_rows = q.part_rows, a.step = q.step, a.parts_per_block = q.per_block;
   a.nparts = q.nparts, a.eps = p->eps;
   hipStream_t st = (hipStream_t)stream;
   const auto run = p->io ? norm<uint16_t> : norm<float>;

@@ -136,6 +136,45 @@ def test_strides(dev, dtype):
             assert mo.rel_l2(p, q) < (1e-2 if dtype == torch.bfloat16 else 1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("gate", ["token", "sequence"])
+@pytest.mark.parametrize("B,T,C", [(1, 1, 9), (2, 2, 13), (3, 6, 20), (2, 7000, 255), (3, 1500, 1531), (1, 3, 4099), (1, 2, 9001)])
+def test_rows_between_boundaries(dev, B, T, C, gate, dtype):
+    """Rows that start anywhere: every array at the same odd place in a buffer of NaN, of which nothing outside the array is
+    taken in or written over; with one array at another place too."""
+    rows, io, f = B * T, dtype == torch.bfloat16, torch.float32
+    gates = rows if gate == "token" else B
+    g = torch.Generator().manual_seed(C)
+
+    def put(n, at, fill=True, dt=dtype):
+        buffer = torch.full((n * C + 32,), float("nan"), dtype=dt, device=dev)
+        if fill:
+            buffer[at:at + n * C] = torch.randn(n * C, generator=g).to(dt).to(dev)
+        return buffer, buffer[at:at + n * C].view(n, C)
+
+    for at, odd in ((3, 3), (0, 0), (3, 2)):
+        x, y, gr, gh = (put(rows, at)[1] for _ in range(4))
+        z = put(gates, odd)[1]
+        w_pre, w_post, scale = (put(1, 5, dt=f)[1][0] for _ in range(3))
+        outs = {n: put(k, at, False) for n, k in (("r", rows), ("h", rows), ("dx", rows), ("dy", rows), ("dgate", gates))}
+        sums = {n: put(1, 5, False, f) for n in ("dw_pre", "dw_post", "dscale")}
+        p = mixers.BlockNorm(io=int(io), rows=rows, C=C, act=mixers.ACTIVATIONS["silu"], gate_rows=1 if gate == "token" else T,
+                             eps=1e-6, x=C, y=C, gate=C, gr=C, gh=C)
+        ptr, stream = (lambda t: t.data_ptr()), torch.cuda.current_stream().cuda_stream
+        L, inputs_ = mixers.lib(), [ptr(t) for t in (x, y, z, w_pre, w_post, scale)]
+        assert L.sffft_blocknorm_fwd(p, *inputs_, ptr(outs["r"][1]), ptr(outs["h"][1]), stream) == 0
+        work = torch.full((L.sffft_blocknorm_work_bytes(p, 1, 1) // 4,), float("nan"), device=dev)
+        assert L.sffft_blocknorm_bwd(p, *inputs_, ptr(gr), ptr(gh), *(ptr(outs[n][1]) for n in ("dx", "dy", "dgate")),
+                                     *(ptr(sums[n][1]) for n in sums), ptr(work), 4 * work.numel(), stream) == 0
+        t = {"x": x, "y": y, "w_pre": w_pre, "w_post": w_post, "gate": z, "scale": scale}
+        shaped = {n: v if v.dim() == 1 else v.view(B, -1, C) for n, v in t.items()}
+        want, grads = oracle(shaped, "silu", gr.view(B, T, C), gh.view(B, T, C))
+        got = [outs["r"], outs["h"]] + [{**outs, **sums}["d" + n] for n in NAMES]
+        for name, (buffer, a), w in zip(("r", "h") + NAMES, got, (*want, *grads)):
+            assert mo.rel_l2(a, w.reshape(a.shape)) < tol(a), (at, odd, name, mo.rel_l2(a, w.reshape(a.shape)))
+            assert int(torch.isnan(buffer).sum()) == 32, (at, odd, name)
+
+
 def test_gradient_against_differences(dev):
     """Central differences of the fp32 kernel's own outputs over a step of 1e-2 of the values: the curvature leaves
     (1e-2)^2 relative, rounding 2^-24 * 1e2 of the sums' sizes: 1e-3 of the gradient's size along the direction."""
