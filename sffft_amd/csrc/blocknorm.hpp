@@ -9,7 +9,7 @@
 // stored value is rounded, and the weights' gradients would be off by that rounding.
 //
 // A row lies in the registers of one workgroup, 8 channels to a lane (16 beyond 8192 channels): every array crosses
-// memory once. A workgroup takes a run of rows and reads the next one before it works on this one (up to 4096 channels);
+// memory once. Rows of up to 256 channels take 16 or 32 lanes of a wavefront, which has several of them. A workgroup takes a run of rows and reads the next one before it works on this one (up to 4096 channels);
 // sums over rows stay in registers until its end, and the parts it leaves are added by a second kernel in a
 // fixed order. Bound by memory: 16384 x 4 rows of 1536 in bf16, gate for each token, 561 us forward and backward for 2.6 GB.
 //
@@ -70,11 +70,18 @@ __device__ __forceinline__ float dpp(float x) {
 __device__ __forceinline__ float lane(float x, int l) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l));
 }
-__device__ __forceinline__ float wave_sum(float x) {
+// Sum over the 16 or 32 lanes of a row.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float x) {
   x += dpp<0xB1>(x);
   x += dpp<0x4E>(x);
   x += dpp<0x141>(x);
   x += dpp<0x140>(x);
+  if constexpr (LANES == 32) x += __shfl_xor(x, 16);
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row_sum<16>(x);
   return (lane(x, 0) + lane(x, 16)) + (lane(x, 32) + lane(x, 48));
 }
 
@@ -83,11 +90,17 @@ __device__ __forceinline__ float wave_sum(float x) {
 struct Sums {
   float v[2][2][16];
 };
+template <int BLK>
 struct Reduce {
   Sums& s;
   int W, turn;
   template <int N>
   __device__ __forceinline__ void operator()(float (&v)[N]) {
+    if constexpr (BLK < 64) {
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = row_sum<BLK>(v[i]);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
     if (W == 1) return;
@@ -106,21 +119,26 @@ struct Reduce {
 };
 
 // Where a lane's N channels lie: vector e of VEC at places (e * lanes + lane) * VEC. The row's channels are the places from
-// `lo` to `hi`: it starts lo elements after a 16-byte boundary. (SHIFT; else lo is 0, and VEC divides C.)
-template <int VEC, int N, bool SHIFT>
+// `lo` to `hi`: it starts lo elements after a 16-byte boundary. (SHIFT; else lo is 0, and VEC divides C.) BLK below 64: the
+// lanes of a row, of which a wavefront has several.
+template <int VEC, int N, int BLK, bool SHIFT>
 struct Places {
+  static constexpr int ROWS = BLK < 64 ? 64 / BLK : 1;  // at once
   int lo, hi;
-  __device__ __forceinline__ int at(int e) const { return (e * (int)blockDim.x + (int)threadIdx.x) * VEC; }
+  __device__ __forceinline__ int at(int e) const {
+    return (BLK < 64 ? e * BLK + (int)threadIdx.x % BLK : e * (int)blockDim.x + (int)threadIdx.x) * VEC;
+  }
+  static __device__ __forceinline__ int row() { return BLK < 64 ? (int)threadIdx.x / BLK : 0; }
   __device__ __forceinline__ bool holds(int place) const { return (!SHIFT || place >= lo) && place < hi; }
   // vector e lies in the row with all its elements
   __device__ __forceinline__ bool whole(int e) const { return !SHIFT || (at(e) >= lo && at(e) + VEC <= hi); }
 };
 
 // A lane's channels of a row, as they are in memory (bf16 two to a register, unless they come one by one).
-template <class T, int VEC, int N, bool SHIFT>
+template <class T, int VEC, int N, int BLK, bool SHIFT>
 struct Row {
   static constexpr int PER = VEC == 1 ? 1 : 4 / (int)sizeof(T), WORDS = VEC / PER;
-  typedef Places<VEC, N, SHIFT> P;
+  typedef Places<VEC, N, BLK, SHIFT> P;
   uint32_t w[N / PER];
   static __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
   static __device__ __forceinline__ uint32_t bits(uint16_t x) { return x; }
@@ -132,14 +150,14 @@ struct Row {
   }
   // `edge`: the array's first or last row. In the others a vector that is not whole is read as a whole, with elements of the
   // neighbouring rows, which mask() clears.
-  __device__ __forceinline__ void load(const void* base, long long row, long long stride, const P& at, bool edge) {
+  __device__ __forceinline__ void load(const void* base, long long row, long long stride, const P& at, bool edge, bool on = true) {
     const T* p = static_cast<const T*>(base) + row * stride - (SHIFT ? at.lo : 0);
 #pragma unroll
     for (int e = 0; e < N / VEC; e++) {
       uint32_t* d = w + e * WORDS;
 #pragma unroll
       for (int i = 0; i < WORDS; i++) d[i] = 0;
-      if (at.at(e) < at.hi) {
+      if (on && at.at(e) < at.hi) {
         if constexpr (VEC == 1) {
           load_elements(p, e, at);
         } else if (SHIFT && edge && !at.whole(e)) {
@@ -173,8 +191,8 @@ struct Row {
     else return __uint_as_float(w[i]);
   }
 };
-template <class T, int VEC, int N, bool SHIFT>
-__device__ __forceinline__ void put_row(void* base, long long row, int C, const Places<VEC, N, SHIFT>& at, const float (&x)[N]) {
+template <class T, int VEC, int N, int BLK, bool SHIFT>
+__device__ __forceinline__ void put_row(void* base, long long row, int C, const Places<VEC, N, BLK, SHIFT>& at, const float (&x)[N]) {
   T* p = static_cast<T*>(base) + row * C - (SHIFT ? at.lo : 0);
 #pragma unroll
   for (int e = 0; e < N / VEC; e++) {
@@ -191,8 +209,8 @@ __device__ __forceinline__ void put_row(void* base, long long row, int C, const 
   }
 }
 // sums, channel by channel where the row is shifted: their rows are aligned in another way
-template <int VEC, int N, bool SHIFT>
-__device__ __forceinline__ void put_sums(float* base, long long part, int C, const Places<VEC, N, SHIFT>& at, const float (&x)[N]) {
+template <int VEC, int N, int BLK, bool SHIFT>
+__device__ __forceinline__ void put_sums(float* base, long long part, int C, const Places<VEC, N, BLK, SHIFT>& at, const float (&x)[N]) {
   if constexpr (!SHIFT) {
     put_row<float>(base, part, C, at, x);
   } else {
@@ -205,8 +223,8 @@ __device__ __forceinline__ void put_sums(float* base, long long part, int C, con
   }
 }
 // weights, 1 where there are none; 0 outside the row
-template <int VEC, int N, bool SHIFT>
-__device__ __forceinline__ void weights(const float* p, const Places<VEC, N, SHIFT>& at, float (&x)[N]) {
+template <int VEC, int N, int BLK, bool SHIFT>
+__device__ __forceinline__ void weights(const float* p, const Places<VEC, N, BLK, SHIFT>& at, float (&x)[N]) {
 #pragma unroll
   for (int e = 0; e < N / VEC; e++) {
     if constexpr (SHIFT) {
@@ -223,10 +241,10 @@ __device__ __forceinline__ void weights(const float* p, const Places<VEC, N, SHI
 }
 
 // What both kernels share: the lane's places, the mask of its elements, and the gates that rows share.
-template <class T, int VEC, int N, bool SHIFT>
+template <class T, int VEC, int N, int BLK, bool SHIFT>
 struct Lane {
-  typedef Row<T, VEC, N, SHIFT> R;
-  Places<VEC, N, SHIFT> at;
+  typedef Row<T, VEC, N, BLK, SHIFT> R;
+  Places<VEC, N, BLK, SHIFT> at;
   uint32_t m[N / R::PER];
   __device__ __forceinline__ Lane(const Args& A, long long first) {
     at.lo = 0;
@@ -248,12 +266,12 @@ struct Lane {
 };
 
 template <class T, int VEC, int N, int BLK, bool SHIFT, bool Y>
-__global__ __launch_bounds__(BLK) void fwd_kernel(Args A) {
+__global__ __launch_bounds__(BLK < 64 ? 64 : BLK, BLK > 512 ? 4 : VEC == 1 || BLK < 64 ? 5 : 6) void fwd_kernel(Args A) {
   constexpr bool AHEAD = BLK <= 512;  // 1024 lanes leave each 128 registers: none for a row in advance
   __shared__ Sums sums;
-  Reduce reduce = {sums, (int)blockDim.x >> 6, 0};
+  Reduce<BLK> reduce = {sums, (int)blockDim.x >> 6, 0};
   const Part part(A, blockIdx.x);
-  Lane<T, VEC, N, SHIFT> lane(A, part.first);
+  Lane<T, VEC, N, BLK, SHIFT> lane(A, part.first);
   const auto& at = lane.at;
   const bool shared = A.gate && A.gate_rows > 1;
   float wq[N], ws[N];
@@ -266,72 +284,70 @@ __global__ __launch_bounds__(BLK) void fwd_kernel(Args A) {
     for (int i = 0; i < N; i++) ws[i] *= sc[i];
   }
   const float inv = 1.f / (float)A.C;
-  Row<T, VEC, N, SHIFT> nx, ny, ng, rg;
+  Row<T, VEC, N, BLK, SHIFT> nx, ny, ng, rg;
+  const long long run = (long long)at.ROWS * A.step;
   auto fetch = [&](long long row) {
-    const bool edge = row == 0 || row == A.rows - 1;
-    nx.load(A.x, row, A.sx, at, edge);
+    row += at.row() * A.step;
+    const bool edge = row == 0 || row == A.rows - 1, on = at.ROWS == 1 || row < part.last;
+    nx.load(A.x, row, A.sx, at, edge, on);
     if constexpr (Y) {
-      ny.load(A.y, row, A.sy, at, edge);
-      if (A.gate && !shared) ng.load(A.gate, row, A.sg, at, edge);
+      ny.load(A.y, row, A.sy, at, edge, on);
+      if (A.gate && !shared) ng.load(A.gate, row, A.sg, at, edge, on);
     }
   };
   if (AHEAD && part.first < part.last) fetch(part.first);
-  long long gate = shared ? part.first / A.gate_rows : 0;  // rows that share one are worked on together
-  for (long long row = part.first; row < part.last; gate++) {
-    long long stop = part.last;
-    if constexpr (Y)
-      if (shared) {
-        lane.gate(A, gate, rg);
-        stop = min(stop, (gate + 1) * A.gate_rows);
-      }
-    for (; row < stop; row += A.step) {
-      if (!AHEAD) fetch(row);
-      Row<T, VEC, N, SHIFT> rx = nx, ry = ny;
-      rx.mask(lane.m);
-      if constexpr (Y) {
-        ry.mask(lane.m);
-        if (!shared) rg = ng, rg.mask(lane.m);
-      }
-      if (AHEAD && row + A.step < part.last) fetch(row + A.step);
-      float x[N], s[1];
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] = rx[i];
-      if constexpr (Y) {
-        float f = 1.f, d;
-        if (A.wp) {
-          s[0] = 0.f;
-#pragma unroll
-          for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
-          reduce(s);
-          f = 1.f / sqrtf(s[0] * inv + A.eps);
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-          float m = ry[i] * f * ws[i];
-          if (A.gate) m *= activate(A.act, rg[i], &d);
-          x[i] += m;
-        }
-        put_row<T>(A.r, row, A.C, at, x);
-      }
-      s[0] = 0.f;
-#pragma unroll
-      for (int i = 0; i < N; i++) s[0] += x[i] * x[i];
-      reduce(s);
-      const float f = 1.f / sqrtf(s[0] * inv + A.eps);
-#pragma unroll
-      for (int i = 0; i < N; i++) x[i] *= f * wq[i];
-      put_row<T>(A.h, row, A.C, at, x);
+  if constexpr (Y)  // rows of a part share theirs
+    if (shared && part.first < part.last) lane.gate(A, part.first / A.gate_rows, rg);
+  for (long long row0 = part.first; row0 < part.last; row0 += run) {
+    if (!AHEAD) fetch(row0);
+    const long long row = row0 + at.row() * A.step;
+    const bool on = at.ROWS == 1 || row < part.last;
+    const float eps = on ? A.eps : 1.f;
+    Row<T, VEC, N, BLK, SHIFT> rx = nx, ry = ny;
+    rx.mask(lane.m);
+    if constexpr (Y) {
+      ry.mask(lane.m);
+      if (!shared) rg = ng, rg.mask(lane.m);
     }
+    if (AHEAD && row0 + run < part.last) fetch(row0 + run);
+    float x[N], s[1];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = rx[i];
+    if constexpr (Y) {
+      float f = 1.f, d;
+      if (A.wp) {
+        s[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
+        reduce(s);
+        f = 1.f / sqrtf(s[0] * inv + eps);
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        float m = ry[i] * f * ws[i];
+        if (A.gate) m *= activate(A.act, rg[i], &d);
+        x[i] += m;
+      }
+      if (on) put_row<T>(A.r, row, A.C, at, x);
+    }
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) s[0] += x[i] * x[i];
+    reduce(s);
+    const float f = 1.f / sqrtf(s[0] * inv + eps);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] *= f * wq[i];
+    if (on) put_row<T>(A.h, row, A.C, at, x);
   }
 }
 
 template <class T, int VEC, int N, int BLK, bool SHIFT, bool Y>
-__global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
+__global__ __launch_bounds__(BLK < 64 ? 64 : BLK) void bwd_kernel(Args A) {
   constexpr bool AHEAD = BLK <= 512;  // 1024 lanes leave each 128 registers: none for a row in advance
   __shared__ Sums sums;
-  Reduce reduce = {sums, (int)blockDim.x >> 6, 0};
+  Reduce<BLK> reduce = {sums, (int)blockDim.x >> 6, 0};
   const Part part(A, blockIdx.x);
-  Lane<T, VEC, N, SHIFT> lane(A, part.first);
+  Lane<T, VEC, N, BLK, SHIFT> lane(A, part.first);
   const auto& at = lane.at;
   const bool shared = A.gate && A.gate_rows > 1;
   const float inv = 1.f / (float)A.C;
@@ -343,32 +359,37 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
     weights(A.wp, at, wp);
     weights(A.sc, at, sc);
   }
-  Row<T, VEC, N, SHIFT> nx, ny, ng, nr, nh;
+  Row<T, VEC, N, BLK, SHIFT> nx, ny, ng, nr, nh;
+  const long long run = (long long)at.ROWS * A.step;
   auto fetch = [&](long long row) {
-    const bool edge = row == 0 || row == A.rows - 1;
-    nx.load(A.x, row, A.sx, at, edge);
+    row += at.row() * A.step;
+    const bool edge = row == 0 || row == A.rows - 1, on = at.ROWS == 1 || row < part.last;
+    nx.load(A.x, row, A.sx, at, edge, on);
     if constexpr (Y) {
-      ny.load(A.y, row, A.sy, at, edge);
-      if (A.gate && !shared) ng.load(A.gate, row, A.sg, at, edge);
+      ny.load(A.y, row, A.sy, at, edge, on);
+      if (A.gate && !shared) ng.load(A.gate, row, A.sg, at, edge, on);
     }
-    if (A.gr) nr.load(A.gr, row, A.sgr, at, edge);
-    if (A.gh) nh.load(A.gh, row, A.sgh, at, edge);
+    if (A.gr) nr.load(A.gr, row, A.sgr, at, edge, on);
+    if (A.gh) nh.load(A.gh, row, A.sgh, at, edge, on);
   };
   if (!A.gr) nr = {};
   if (!A.gh) nh = {};
   if (AHEAD && part.first < part.last) fetch(part.first);
-  Row<T, VEC, N, SHIFT> rg = {};
+  Row<T, VEC, N, BLK, SHIFT> rg = {};
   if constexpr (Y)  // rows of a part share theirs
     if (shared && part.first < part.last) lane.gate(A, part.first / A.gate_rows, rg);
-  for (long long row = part.first; row < part.last; row += A.step) {
-    if (!AHEAD) fetch(row);
-    Row<T, VEC, N, SHIFT> rx = nx, ry = ny, rr = nr, rh = nh;
+  for (long long row0 = part.first; row0 < part.last; row0 += run) {
+    if (!AHEAD) fetch(row0);
+    const long long row = row0 + at.row() * A.step;
+    const bool on = at.ROWS == 1 || row < part.last;
+    const float eps = on ? A.eps : 1.f;
+    Row<T, VEC, N, BLK, SHIFT> rx = nx, ry = ny, rr = nr, rh = nh;
     rx.mask(lane.m), rr.mask(lane.m), rh.mask(lane.m);
     if constexpr (Y) {
       ry.mask(lane.m);
       if (!shared) rg = ng, rg.mask(lane.m);
     }
-    if (AHEAD && row + A.step < part.last) fetch(row + A.step);
+    if (AHEAD && row0 + run < part.last) fetch(row0 + run);
     float r[N], y[N], act[N], s[1], fy = 1.f, d;
 #pragma unroll
     for (int i = 0; i < N; i++) r[i] = rx[i];
@@ -378,7 +399,7 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
 #pragma unroll
         for (int i = 0; i < N; i++) s[0] += ry[i] * ry[i];
         reduce(s);
-        fy = 1.f / sqrtf(s[0] * inv + A.eps);
+        fy = 1.f / sqrtf(s[0] * inv + eps);
       }
 #pragma unroll
       for (int i = 0; i < N; i++) {
@@ -391,7 +412,7 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
 #pragma unroll
     for (int i = 0; i < N; i++) q[0] += r[i] * r[i], q[1] += rh[i] * wq[i] * r[i];
     reduce(q);
-    const float fr = 1.f / sqrtf(q[0] * inv + A.eps), mean = q[1] * fr * inv;
+    const float fr = 1.f / sqrtf(q[0] * inv + eps), mean = q[1] * fr * inv;
     float dr[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -399,7 +420,7 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
       dwq[i] += rh[i] * r[i];
       dr[i] = rr[i] + fr * (rh[i] * wq[i] - r[i] * mean);
     }
-    put_row<T>(A.dx, row, A.C, at, dr);
+    if (on) put_row<T>(A.dx, row, A.C, at, dr);
     if constexpr (Y) {
       if (shared) {
 #pragma unroll
@@ -415,7 +436,7 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
           activate(A.act, rg[i], &d);
           g[i] = dr[i] * sc[i] * y[i] * wp[i] * d;
         }
-        put_row<T>(A.dgate, row, A.C, at, g);
+        if (on) put_row<T>(A.dgate, row, A.C, at, g);
       }
 #pragma unroll
       for (int i = 0; i < N; i++) dr[i] *= sc[i] * act[i];
@@ -431,8 +452,18 @@ __global__ __launch_bounds__(BLK) void bwd_kernel(Args A) {
 #pragma unroll
         for (int i = 0; i < N; i++) dr[i] = fy * (dr[i] - y[i] * my);
       }
-      put_row<T>(A.dy, row, A.C, at, dr);
+      if (on) put_row<T>(A.dy, row, A.C, at, dr);
     }
+  }
+  if constexpr (BLK < 64) {  // the sums of a wavefront's rows
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int o = BLK; o < 64; o *= 2) {
+        dwq[i] += __shfl_xor(dwq[i], o);
+        if constexpr (Y) t[i] += __shfl_xor(t[i], o);
+      }
+    if (at.row()) return;
   }
   put_sums(A.parts, blockIdx.x, A.C, at, dwq);
   if constexpr (Y) {

@@ -58,12 +58,13 @@ enum Access { WHOLE, HALVES, SHIFTED, SINGLE };
 struct RowShape {
   Access access;
   int n, waves, step;
+  int lanes;  // of a row, where a wavefront has several: 16 or 32; else 64
 };
 RowShape row_shape(const sffft_blocknorm* p, Access access) {
   const int V = p->io ? 8 : 4, places = p->C + (access == SHIFTED ? V - 1 : 0), n = places > 8192 ? 16 : 8;
   int step = 1;
   while (access == SHIFTED && (long long)step * p->C % V) step *= 2;
-  return {access, n, (places + 64 * n - 1) / (64 * n), step};
+  return {access, n, (places + 64 * n - 1) / (64 * n), step, places <= 128 ? 16 : places <= 256 ? 32 : 64};
 }
 constexpr int MAX_WAVES = 16;
 
@@ -80,7 +81,8 @@ Parts parts_of(const sffft_blocknorm* p, const RowShape& s, bool shared_gate, in
   q.step = (int)std::min<long long>(s.step, q.block_rows);
   const long long groups = std::max<long long>(1, 256 * std::max(1, fill / s.waves) / q.blocks / q.step);
   const long long run = (q.block_rows + q.step - 1) / q.step;  // rows of a class
-  q.part_rows = (int)std::min<long long>((run + groups - 1) / groups, INT_MAX / 16);
+  const long long rows = 64 / s.lanes, each = (run + groups - 1) / groups;
+  q.part_rows = (int)std::min<long long>((each + rows - 1) / rows * rows, INT_MAX / 16);
   q.per_block = (int)std::min<long long>((run + q.part_rows - 1) / q.part_rows * q.step, INT_MAX);
   q.nparts = q.blocks * q.per_block;
   return q;
@@ -101,7 +103,9 @@ void norm_launch(const bn::Args& a, int waves, bool y, bool backward, dim3 grid,
 }
 template <class T, int VEC, bool SHIFT = false>
 void norm_access(const bn::Args& a, const RowShape& s, bool y, bool backward, dim3 grid, hipStream_t st) {
-  if (s.n == 16) norm_launch<T, VEC, 16, 1024, SHIFT>(a, s.waves, y, backward, grid, st);
+  if (s.lanes == 16) norm_launch<T, VEC, 8, 16, SHIFT>(a, s.waves, y, backward, grid, st);
+  else if (s.lanes == 32) norm_launch<T, VEC, 8, 32, SHIFT>(a, s.waves, y, backward, grid, st);
+  else if (s.n == 16) norm_launch<T, VEC, 16, 1024, SHIFT>(a, s.waves, y, backward, grid, st);
   else if (s.waves > 8) norm_launch<T, VEC, 8, 1024, SHIFT>(a, s.waves, y, backward, grid, st);
   else if (s.waves > 4) norm_launch<T, VEC, 8, 512, SHIFT>(a, s.waves, y, backward, grid, st);
   else norm_launch<T, VEC, 8, 256, SHIFT>(a, s.waves, y, backward, grid, st);
@@ -270,7 +274,7 @@ int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, 
   if (!ops::aligned(r, elem) || !ops::aligned(h, elem) || !apart(in, 6, out, 2)) return SFFFT_EINVAL;
   const RowShape s = row_shape(p, access_of(p, {{x, p->x}, {y, p->y}, {r, p->C}, {h, p->C}}, {gate, p->gate},
                                             {w_pre, w_post, scale}));
-  const Parts q = parts_of(p, s, false, FILL_FWD);
+  const Parts q = parts_of(p, s, gate && p->gate_rows > 1, FILL_FWD);
   if (q.nparts > INT_MAX) return SFFFT_EINVAL;
   bn::Args a = {};
   a.x = x, a.y = y, a.gate = gate, a.sx = p->x, a.sy = p->y, a.sg = p->gate;

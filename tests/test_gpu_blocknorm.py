@@ -175,6 +175,22 @@ def test_rows_between_boundaries(dev, B, T, C, gate, dtype):
             assert int(torch.isnan(buffer).sum()) == 32, (at, odd, name)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("gate", ["token", "sequence", "none"])
+@pytest.mark.parametrize("B,T,C", [(1, 1, 2), (5, 3, 8), (2, 77, 37), (3, 41, 64), (2, 5, 100), (1, 1001, 121), (2, 333, 128), (3, 35, 129),
+                                   (1, 9, 200), (2, 50, 249), (1, 70, 256), (2, 70000, 64)])
+def test_several_rows_to_a_wavefront(dev, B, T, C, gate, dtype):
+    """Narrow rows, and counts of them that leave some lanes without one; eps = 0, where the norm of nothing is not defined."""
+    t, gr, gh = inputs(dev, (B, T, C), dtype, gate, seed=C)
+    want, wgrads = oracle(t, "sigmoid", gr, gh, 0.0)
+    out, grads = run(t, "sigmoid", gr, gh, 0.0)
+    names = ("r", "h", *[n for n in NAMES if t[n] is not None])
+    for name, a, w in zip(names, (*out, *grads), (*want, *wgrads)):
+        assert a.shape == w.shape and mo.rel_l2(a, w) < tol(a), (name, mo.rel_l2(a, w))
+    h = torch.ops.sffft.pre_norm(t["x"], t["w_pre"], 0.0)
+    assert mo.rel_l2(h, mo.block_norm(t["x"].double().cpu(), None, t["w_pre"].double().cpu(), None, None, None, "none", 0.0)[1]) < tol(h)
+
+
 def test_gradient_against_differences(dev):
     """Central differences of the fp32 kernel's own outputs over a step of 1e-2 of the values: the curvature leaves
     (1e-2)^2 relative, rounding 2^-24 * 1e2 of the sums' sizes: 1e-3 of the gradient's size along the direction."""
