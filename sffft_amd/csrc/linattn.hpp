@@ -275,9 +275,11 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   auto power = [&](int n) { return n < 0 ? 0.f : __builtin_amdgcn_exp2f(l2 * (float)n); };
   auto count = [&](int t0) { return __builtin_amdgcn_readfirstlane(min(max(end - t0, 0), C)); };
 
-  // the first chunk: the last one of the segment if reversed
-  const int dir = rev ? -C : C;
-  int t0 = rev ? first + (chunks - 1) * C : first;
+  // The first chunk: the last one of the segment if reversed. The sums go the other way, so that what they read last is what
+  // the march reads first, out of the cache that all XCDs share.
+  const bool back = OUT ? rev : !rev;
+  const int dir = back ? -C : C;
+  int t0 = back ? first + (chunks - 1) * C : first;
   const T* pa = static_cast<const T*>(m.a.p) + b * m.a.sb + (h / m.a.div) * m.a.sh + t0 * m.a.st;
   const T* pb = static_cast<const T*>(m.b.p) + b * m.b.sb + (h / m.b.div) * m.b.sh + t0 * m.b.st;
   const T* pc = static_cast<const T*>(m.c.p) + b * m.c.sb + (h / m.c.div) * m.c.sh + t0 * m.c.st + v0;
@@ -425,7 +427,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   };
 
   float gn = 1.f;
-  int have = -1;
+  int have = OUT ? -1 : 0;  // tokens of the chunk that the decays are for; of the chunks before
   for (int c = 0; c < chunks; c++) {
     ops::barrier();
     if constexpr (OUT) {  // the last chunk's
@@ -436,14 +438,15 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
     }
     gb.store(tb);
     gc.store(tc);
-    if (n != have) {  // the decays depend on the tokens in a chunk
-      have = n;
-      gn = power(n);
-      const int i = threadIdx.x;
+    // The decays depend on the tokens in a chunk; in the sums also on those between the chunk and where the sum is taken.
+    if (!OUT || n != have) {
+      const int i = threadIdx.x, behind = OUT ? 0 : have;
       if (i < C) {
-        fi[i] = m.x * power(rev ? n - 1 - i : i + 1);
-        wj[i] = m.w * power(i >= n ? -1 : rev ? i + 1 : n - 1 - i);
+        if constexpr (OUT) fi[i] = m.x * power(rev ? n - 1 - i : i + 1);
+        wj[i] = m.w * power(i >= n ? -1 : behind + (rev ? i + 1 : n - 1 - i));
       }
+      if constexpr (OUT) have = n, gn = power(n);
+      else have += n;
     }
     t0 += dir;
     n = c + 1 < chunks ? count(t0) : 0;  // past the last chunk nothing is valid, and nothing is read
@@ -503,10 +506,11 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
       ops::barrier();
     }
 
+    if constexpr (OUT)
 #pragma unroll
-    for (int a = 0; a < KA; a++)
+      for (int a = 0; a < KA; a++)
 #pragma unroll
-      for (int v = 0; v < VW; v++) S[a][v] *= gn;
+        for (int v = 0; v < VW; v++) S[a][v] *= gn;
 #pragma unroll
     for (int s = 0; s < JS; s++) {
       // c's channels as an operand, tokens along the sum; and decayed, to be added to the state
