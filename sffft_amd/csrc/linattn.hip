@@ -37,7 +37,13 @@ bool valid_input(const void* x, const long long s[3], const sffft_linattn* p, in
 
 Operand operand(const void* x, const long long s[3], int div) { return {x, s[0], s[1], s[2], div}; }
 
-// How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march.
+// More segments than this are joined by a launch of its own, fewer by each workgroup that follows them.
+constexpr int MAX_JOINED = 8;
+
+// How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march. No more than MAX_JOINED
+// where these still come near filling the chip and are few chunks longer: a launch and the states' way through memory less.
+// (us, bf16, 64 channels: 4 x 12 heads of 600 tokens 22.4 -> 17.3, 5 x 12 of 2048 39.4 -> 30.8, 2 x 12 of 2048 29.5 -> 24.4, but of 8192 45.6
+// -> 57; 128 channels: 4 x 12 of 600 40.4 -> 34.5, 8 of 1000 26.7 -> 30.7.)
 struct Cut {
   int nseg, seg;
 };
@@ -46,7 +52,9 @@ Cut cut_of(const sffft_linattn* p, int marches) {
   const int chunks = (p->T + C - 1) / C, fill = D > 64 ? 512 : 1024;
   const long long heads = (long long)p->B * p->H * marches;
   const int want = (int)std::min<long long>(chunks, std::max<long long>(1, fill / heads));
-  const int per = (chunks + want - 1) / want;
+  const int few = (chunks + MAX_JOINED - 1) / MAX_JOINED, joined = (chunks + few - 1) / few;
+  int per = (chunks + want - 1) / want;
+  if (few > per && few - per <= (D > 64 ? 1 : 3) && joined * heads >= (D > 64 ? 240 : 192)) per = few;
   return {(chunks + per - 1) / per, per * C};
 }
 
@@ -97,8 +105,6 @@ hipError_t head_sum(const float* in, void* out, long long n, int D, int G, hipSt
 size_t state_bytes(const sffft_linattn* p, const Cut& c) {
   return c.nseg == 1 ? 0 : (size_t)p->B * p->H * c.nseg * p->Dk * p->Dv * 4;
 }
-// More segments than this are joined by a launch of its own, fewer by each workgroup that follows them.
-constexpr int MAX_JOINED = 8;
 // From this many segments on the sum of the last one is made too, for the last state: it costs one more of many sums, and the
 // march then adds to its state only what outputs of 16 bits need.
 constexpr int MIN_ALL = 4;
