@@ -151,16 +151,18 @@ __device__ __forceinline__ Frag<NS> split8(const float (&x)[8]) {
 }
 
 // Row-major [C][L] tiles of 16 bits in LDS, NS planes. Rows are padded by 32 bytes: the transposing reads below
-// touch 8 rows of 32 bytes at a time, on 64 different banks.
-template <int NS, int C, int L>
+// touch 8 rows of 32 bytes at a time, on 64 different banks. SWAP: in rows 8..15 of each 16 neighbouring pieces of 16 bytes change
+// places, so that reads of a piece of 16 rows find 64 different banks too (the 8 rows' starts are 8 banks apart).
+template <int NS, int C, int L, bool SWAP = true>
 struct Tile {
   u16 v[NS][C][L];
+  static __device__ __forceinline__ int at(int row, int col) { return SWAP ? col ^ (row & 8) : col; }
 
   // operand whose index is the row: lane (g, i) holds channels at..at+7 of row r0 + i, at = c0 + 8 g
   __device__ __forceinline__ Frag<NS> rows(int r0, int c0, int i, int g) const {
     Frag<NS> f;
 #pragma unroll
-    for (int p = 0; p < NS; p++) f.p[p] = *reinterpret_cast<const bf16x8*>(&v[p][r0 + i][c0 + 8 * g]);
+    for (int p = 0; p < NS; p++) f.p[p] = *reinterpret_cast<const bf16x8*>(&v[p][r0 + i][c0 + at(i, 8 * g)]);
     return f;
   }
   // the same with the channels in the order of an accumulator's rows: c0 + 4 g .. + 3 and c0 + 16 + 4 g .. + 3
@@ -168,8 +170,8 @@ struct Tile {
     Frag<NS> f;
 #pragma unroll
     for (int p = 0; p < NS; p++) {
-      const uint2 a = *reinterpret_cast<const uint2*>(&v[p][r0 + i][c0 + 4 * g]);
-      const uint2 b = *reinterpret_cast<const uint2*>(&v[p][r0 + i][c0 + 16 + 4 * g]);
+      const uint2 a = *reinterpret_cast<const uint2*>(&v[p][r0 + i][c0 + at(i, 4 * g)]);
+      const uint2 b = *reinterpret_cast<const uint2*>(&v[p][r0 + i][c0 + 16 + at(i, 4 * g)]);
       f.p[p] = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
     }
     return f;
@@ -181,7 +183,7 @@ struct Tile {
     Frag<NS> f;
 #pragma unroll
     for (int p = 0; p < NS; p++) {
-      const u16* q = &v[p][r0 + 4 * g + (i >> 2)][c0 + 4 * (i & 3)];
+      const u16* q = &v[p][r0 + 4 * g + (i >> 2)][c0 + at(4 * g, 4 * (i & 3))];
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q);
       const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 16 * L));
       const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
@@ -206,8 +208,14 @@ struct Stage {
   static constexpr int E = 16 / sizeof(T), PER = DT / E, N = C * PER / 256, ROWS = 256 / PER;
   static constexpr uint32_t RECORDS = 0x7fffffffu, OUTSIDE = 0x80000000u;
   i32x4 v[N];
+  // The lane's row among ROWS. Rows of 128 bytes are written two at a time: 4 apart they lie on different banks.
+  static __device__ __forceinline__ int row() {
+    const int r = threadIdx.x / PER;
+    return PER * sizeof(T) * E == 128 && sizeof(T) == 2 ? (r & ~7) | (r & 1) << 2 | (r & 6) >> 1 : r;
+  }
+  static __device__ __forceinline__ int col() { return threadIdx.x % PER * E; }
   __device__ __forceinline__ void load(const T* p, long long st, int n, int D) {
-    const int row = threadIdx.x / PER, col = threadIdx.x % PER * E;
+    const int row = this->row(), col = this->col();
     const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, RECORDS, 0x00027000);
     const uint32_t at = col < D ? (uint32_t)(row * (int)st + col) * sizeof(T) : OUTSIDE;
 #pragma unroll
@@ -218,7 +226,7 @@ struct Stage {
   __device__ __forceinline__ void store(Tile<NS, C, L>& t) const {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int row = threadIdx.x / PER + i * ROWS, col = threadIdx.x % PER * E;
+      const int row = this->row() + i * ROWS, col = t.at(row, this->col());
       if constexpr (NS == 1) {
         *reinterpret_cast<i32x4*>(&t.v[0][row][col]) = v[i];
       } else {
@@ -252,7 +260,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, KT + 16> ta;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, KT + 16> tb;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, VT + 16> tc;
-  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, C + 8> tp;
+  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, C + 8, false> tp;
   __shared__ __attribute__((aligned(16))) float fi[C], wj[C];  // decays: of the entering state at row i, of token j in the update
 
   // Workgroups go to the 8 XCDs in turn; the marches and V tiles of one head and segment, which read the same
@@ -392,18 +400,18 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
       for (int t = 0; t < MT; t++)
 #pragma unroll
         for (int v = 0; v < VW; v++)
-          *reinterpret_cast<uint2*>(&ta.v[0][16 * t + i16][16 * (w * VW + v) + 4 * g]) =
+          *reinterpret_cast<uint2*>(&ta.v[0][16 * t + i16][16 * (w * VW + v) + ta.at(i16, 4 * g)]) =
               make_uint2(ops::pack_bf16(o[t][v][0], o[t][v][1]), ops::pack_bf16(o[t][v][2], o[t][v][3]));
   };
   auto store_out = [&]() {
     if constexpr (VIA) {
       typedef Stage<T, C, VT> G;
       const auto r = __builtin_amdgcn_make_buffer_rsrc(po + v0, 0, 0x7fffffff, 0x00027000);
-      const int row = threadIdx.x / G::PER, col = threadIdx.x % G::PER * G::E;
+      const int row = G::row(), col = G::col();
       const uint32_t at = v0 + col < m.V ? (uint32_t)(row * orow + col) * E : 0x80000000u;
 #pragma unroll
       for (int i = 0; i < G::N; i++) {
-        const i32x4 x = *reinterpret_cast<const i32x4*>(&ta.v[0][row + i * G::ROWS][col]);
+        const i32x4 x = *reinterpret_cast<const i32x4*>(&ta.v[0][row + i * G::ROWS][ta.at(row + i * G::ROWS, col)]);
         store16(x, r, row + i * G::ROWS < left ? at + i * G::ROWS * orow * E : 0x80000000u);
       }
     } else {
