@@ -31,7 +31,9 @@ extern "C" {
  * S_{-1} is the initial state (zero if NULL); the final state is S_{n-1} (the initial one if n = 0).
  * States are [B][H][Dk][Dv] fp32. Tokens from n on are never read, whatever they hold. log_decay
  * <= 0 is meant (-inf: nothing is remembered); a positive one grows until it overflows. lengths
- * outside 0..T are taken as the nearest of these. */
+ * outside 0..T are taken as the nearest of these. Tokens are worked on in chunks of 64 (fp32: 32): an
+ * infinity or NaN at one that counts may make NaN of the outputs of its whole chunk, and does of the later
+ * ones; an infinity in fp32 counts as NaN. */
 typedef struct sffft_linattn {
   int io;                 /* SFFFT_IO_F32 or SFFFT_IO_BF16: q, k, v, o and their gradients */
   int B, T, H, Hk;        /* H a multiple of Hk, at most 2^23 - 64 channels in all its heads */
@@ -72,8 +74,8 @@ int sffft_linattn_step(const sffft_linattn* p, const void* q, const void* k, con
  * interleaved:  a' = a cos - b sin,  b' = b cos + a sin; channels from R on are copied. With
  * inverse = 1 by the negative angle (the gradient). Token t of sequence b has position
  * pos[b][t] (pos_bits 32 or 64), t if pos is NULL; a position outside the table gives NaN in the
- * rotated channels and reads nothing. (H + Hk) * D / 2 is at most 65535. qo may be q and ko k, with equal strides; else they overlap
- * neither. */
+ * rotated channels and reads nothing. (H + Hk) * D / 2 is at most 65535. qo may be q and ko k, with
+ * equal strides; else they overlap neither. */
 typedef struct sffft_rotary {
   int io;
   int B, T, H, Hk, D;

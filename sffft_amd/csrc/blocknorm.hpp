@@ -9,13 +9,14 @@
 // stored value is rounded, and the weights' gradients would be off by that rounding.
 //
 // A row lies in the registers of one workgroup, 8 channels to a lane (16 beyond 8192 channels): every array crosses
-// memory once. Rows of up to 256 channels take 16 or 32 lanes of a wavefront, which has several of them. A workgroup takes a run of rows and reads the next one before it works on this one (up to 4096 channels);
-// sums over rows stay in registers until its end, and the parts it leaves are added by a second kernel in a
-// fixed order. Bound by memory: 16384 x 4 rows of 1536 in bf16, gate for each token, 561 us forward and backward for 2.6 GB.
+// memory once. Rows of up to 256 channels take 16 or 32 lanes of a wavefront, which has several of them. A workgroup
+// takes a run of rows and reads the next one before it works on this one (up to 4096 channels); sums over rows stay
+// in registers until its end, and the parts it leaves are added by a second kernel in a fixed order. Bound by memory:
+// 16384 x 4 rows of 1536 in bf16, gate for each token, 561 us forward and backward for 2.6 GB.
 //
-// Rows of an odd width start anywhere between 16-byte boundaries. A workgroup then takes rows that start at the same distance from one
-// (every 2nd, 4th or 8th) and reads them from the boundary before the row on: the vectors stay aligned and the
-// lane's channels the same in all its rows, so that the sums over rows stay in registers.
+// Rows of an odd width start anywhere between 16-byte boundaries. A workgroup then takes rows that start at the same
+// distance from one (every 2nd, 4th or 8th) and reads them from the boundary before the row on: the vectors stay
+// aligned and the lane's channels the same in all its rows, so that the sums over rows stay in registers.
 #pragma once
 #include "opsio.hpp"
 
@@ -118,9 +119,9 @@ struct Reduce {
   }
 };
 
-// Where a lane's N channels lie: vector e of VEC at places (e * lanes + lane) * VEC. The row's channels are the places from
-// `lo` to `hi`: it starts lo elements after a 16-byte boundary. (SHIFT; else lo is 0, and VEC divides C.) BLK below 64: the
-// lanes of a row, of which a wavefront has several.
+// Where a lane's N channels lie: vector e of VEC at places (e * lanes + lane) * VEC. The row's channels are the
+// places from `lo` to `hi`: it starts lo elements after a 16-byte boundary. (SHIFT; else lo is 0, and VEC divides C.)
+// BLK below 64: the lanes of a row, of which a wavefront has several.
 template <int VEC, int N, int BLK, bool SHIFT>
 struct Places {
   static constexpr int ROWS = BLK < 64 ? 64 / BLK : 1;  // at once
@@ -148,8 +149,8 @@ struct Row {
     for (int i = 0; i < VEC; i++)
       if (at.holds(at.at(e) + i)) w[(e * VEC + i) / PER] |= bits(p[at.at(e) + i]) << (sizeof(T) == 4 ? 0 : PER == 1 ? 16 : 16 * (i & 1));
   }
-  // `edge`: the array's first or last row. In the others a vector that is not whole is read as a whole, with elements of the
-  // neighbouring rows, which mask() clears.
+  // `edge`: the array's first or last row. In the others a vector that is not whole is read as a whole, with elements
+  // of the neighbouring rows, which mask() clears.
   __device__ __forceinline__ void load(const void* base, long long row, long long stride, const P& at, bool edge, bool on = true) {
     const T* p = static_cast<const T*>(base) + row * stride - (SHIFT ? at.lo : 0);
 #pragma unroll

@@ -37,13 +37,17 @@ bool valid_input(const void* x, const long long s[3], const sffft_linattn* p, in
 
 Operand operand(const void* x, const long long s[3], int div) { return {x, s[0], s[1], s[2], div}; }
 
-// More segments than this are joined by a launch of its own, fewer by each workgroup that follows them.
+// More segments than this are joined by a launch of its own, fewer by each workgroup that follows them. (us at 4, 8,
+// 16: training, 8 x 2048 tokens, 12 heads of 64 channels, bf16 118.5, 114.1, 114.3; 5 x 1237 tokens forward 24.3,
+// 24.5, 27.4; training, 3 x 1531 tokens, 12 heads on 4 of 96 and 64, fp32 164.3, 162.2, 188.4.)
 constexpr int MAX_JOINED = 8;
 
-// How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march. No more than MAX_JOINED
-// where these still come near filling the chip and are few chunks longer: a launch and the states' way through memory less.
-// (us, bf16, 64 channels: 4 x 12 heads of 600 tokens 22.4 -> 17.3, 5 x 12 of 2048 39.4 -> 30.8, 2 x 12 of 2048 29.5 -> 24.4, but of 8192 45.6
-// -> 57; 128 channels: 4 x 12 of 600 40.4 -> 34.5, 8 of 1000 26.7 -> 30.7.)
+// How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march, two or three
+// to a CU by their registers (half, these, double: the training step above 116.4, 114.1, 121.3; 131072 tokens of 12
+// heads of 128 channels 586, 549, 595). No more than MAX_JOINED where these still come near filling the chip and are
+// few chunks longer: a launch and the states' way through memory less. (us, bf16, 64 channels: 4 x 12 heads of 600
+// tokens 22.4 -> 17.3, 5 x 12 of 2048 39.4 -> 30.8, 2 x 12 of 2048 29.5 -> 24.4, but of 8192 45.6 -> 57; 128
+// channels: 4 x 12 of 600 40.4 -> 34.5, 8 of 1000 26.7 -> 30.7.)
 struct Cut {
   int nseg, seg;
 };
@@ -58,7 +62,8 @@ Cut cut_of(const sffft_linattn* p, int marches) {
   return {(chunks + per - 1) / per, per * C};
 }
 
-// Marches of the gradients' smallest launch (see backward): they share one where sizes and types are equal.
+// Marches of the gradients' smallest launch (see backward): they share one where sizes and types are equal. (Segments
+// for three marches also where each has a launch of its own: the fp32 step above 196 us instead of 162.)
 int backward_marches(const sffft_linattn* p) { return p->Dk == p->Dv && (p->H == p->Hk || !p->io) ? 3 : 1; }
 
 template <class T, class TO, int KT, int VT, bool OUT, int UP>
@@ -71,6 +76,7 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
   return hipGetLastError();
 }
 // Tiles of 64 or 128 channels. fp32 takes 64 of V: the planes of 128 leave no room for a second workgroup on a CU.
+// (bf16, two tiles of 64 of V instead of one of 128: 700 us against 570 for 131072 tokens.)
 template <class T, class TO, bool OUT, int UP>
 hipError_t march_planes(la::Launch& L, hipStream_t st) {
   const int K = L.m[0].K, V = L.m[0].V;
@@ -105,8 +111,9 @@ hipError_t head_sum(const float* in, void* out, long long n, int D, int G, hipSt
 size_t state_bytes(const sffft_linattn* p, const Cut& c) {
   return c.nseg == 1 ? 0 : (size_t)p->B * p->H * c.nseg * p->Dk * p->Dv * 4;
 }
-// From this many segments on the sum of the last one is made too, for the last state: it costs one more of many sums, and the
-// march then adds to its state only what outputs of 16 bits need.
+// From this many segments on the sum of the last one is made too, for the last state: it costs one more of many sums,
+// and the march then adds to its state only what outputs of 16 bits need. (Never: 115.4, 25.1 and 164 us in the cases
+// above.)
 constexpr int MIN_ALL = 4;
 // dk and dv of heads that are shared, for each query head, before their sum
 size_t shared_bytes(const sffft_linattn* p) {

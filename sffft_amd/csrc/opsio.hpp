@@ -21,8 +21,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(uint16_t* p, float x) { *p = (uint16_t)pack_bf16(x, x); }
 
-// __syncthreads with its wait for LDS written out: at the head of a loop the compiler weakened the one it inserts to none,
-// with LDS writes of the loop's end still outstanding. (0xc07f: lgkmcnt 0, the other counters not waited for.)
+// __syncthreads with its wait for LDS written out: at the head of a loop the compiler weakened the one it inserts to
+// none, with LDS writes of the loop's end still outstanding. (0xc07f: lgkmcnt 0, the other counters not waited for.)
 __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
   __builtin_amdgcn_s_waitcnt(0xc07f);
