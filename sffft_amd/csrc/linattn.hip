@@ -83,6 +83,7 @@ hipError_t march_planes(la::Launch& L, hipStream_t st) {
   if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 2)
     if (V > 64) return launch<T, TO, 128, 128, OUT, UP>(L, st);
+  if (K <= 96) return launch<T, TO, 96, 64, OUT, UP>(L, st);
   return launch<T, TO, 128, 64, OUT, UP>(L, st);
 }
 // nm marches of the same K and V
@@ -101,9 +102,11 @@ hipError_t scan(const la::ScanLaunch& L, int n, hipStream_t st) {
 }
 
 template <class T>
-hipError_t head_sum(const float* in, void* out, long long n, int D, int G, hipStream_t st) {
-  hipLaunchKernelGGL(la::head_sum_kernel<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, in,
-                     static_cast<T*>(out), n, D, G);
+hipError_t head_sums(la::HeadSums L, hipStream_t st) {
+  unsigned blocks[2];
+  for (int i = 0; i < 2; i++) blocks[i] = (unsigned)((L.s[i].n / 4 + 255) / 256);
+  L.blocks = blocks[0];
+  hipLaunchKernelGGL(la::head_sum_kernel<T>, dim3(blocks[0] + blocks[1]), dim3(256), 0, st, L);
   return hipGetLastError();
 }
 
@@ -174,10 +177,8 @@ hipError_t backward(const sffft_linattn* p, const void* q, const void* k, const 
     if (!split) run({mq, mk}, false), run({mv}, false);
     else run({mq}, false), run({mk}, true), run({mv}, true);
   }
-  if (!parts) return e;
-  if (e == hipSuccess) e = head_sum<T>(wk, dk, (long long)rows * p->Hk * Dk, Dk, G, st);
-  if (e == hipSuccess) e = head_sum<T>(wv, dv, (long long)rows * p->Hk * Dv, Dv, G, st);
-  return e;
+  if (!parts || e != hipSuccess) return e;
+  return head_sums<T>({{{wk, dk, (long long)rows * p->Hk * Dk, Dk}, {wv, dv, (long long)rows * p->Hk * Dv, Dv}}, G, 0}, st);
 }
 
 }  // namespace

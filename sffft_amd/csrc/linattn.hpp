@@ -230,11 +230,14 @@ struct Stage {
     for (int i = 0; i < N; i++)
       v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, row + i * ROWS < n ? at : OUTSIDE, i * ROWS * (int)st * (int)sizeof(T), 0);
   }
+  // (tiles of 96 channels are fetched by the lanes of 128)
   template <int NS, int L>
   __device__ __forceinline__ void store(Tile<NS, C, L>& t) const {
+    constexpr int W = L - 16;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int row = this->row() + i * ROWS, col = t.at(row, this->col());
+      if (DT > W && this->col() >= W) break;
       if constexpr (NS == 1) {
         *reinterpret_cast<i32x4*>(&t.v[0][row][col]) = v[i];
       } else {
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   const int orow = L.s.H * m.V;
   TO* po = OUT ? static_cast<TO*>(m.out) + (((long long)b * L.s.T + t0) * L.s.H + h) * m.V : nullptr;
 
-  Stage<T, C, KT> ga, gb;
+  Stage<T, C, KT == 96 ? 128 : KT> ga, gb;
   Stage<T, C, VT> gc;
   auto fetch = [&](int n) {
     if constexpr (OUT) ga.load(pa, m.a.st, n, m.K);
@@ -616,13 +619,27 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
   if (c.s1) ops::store(c.s1 + (long long)bh * c.n + e, x);
 }
 
-// Sum over the query heads that share a key/value head: out [rows][Hk][D] from in [rows][H][D].
+// Sums over the query heads that share a key/value head, of dk and of dv: out [rows][Hk][D] from in [rows][H][D].
+struct HeadSum {
+  const float* in;
+  void* out;
+  long long n;
+  int D;
+};
+struct HeadSums {
+  HeadSum s[2];
+  int G;
+  unsigned blocks;  // workgroups of the first
+};
 template <class T>
-__global__ __launch_bounds__(256) void head_sum_kernel(const float* in, T* out, long long n, int D, int G) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
+__global__ __launch_bounds__(256) void head_sum_kernel(HeadSums L) {
+  const bool second = blockIdx.x >= L.blocks;
+  const HeadSum& A = L.s[second];
+  const int D = A.D, G = L.G;
+  const long long i = ((long long)(blockIdx.x - (second ? L.blocks : 0)) * 256 + threadIdx.x) * 4;
+  if (i >= A.n) return;
   const long long head = i / D;
-  const float* p = in + head * G * D + (i - head * D);
+  const float* p = A.in + head * G * D + (i - head * D);
   float x[4] = {0.f, 0.f, 0.f, 0.f};
   for (int g = 0; g < G; g++) {
     float y[4];
@@ -630,7 +647,7 @@ __global__ __launch_bounds__(256) void head_sum_kernel(const float* in, T* out, 
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] += y[e];
   }
-  ops::store(out + i, x);
+  ops::store(static_cast<T*>(A.out) + i, x);
 }
 
 // One token: lane (r, c) takes four columns c of rows r, r + 16, ... of the state.

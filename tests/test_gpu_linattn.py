@@ -113,6 +113,25 @@ def test_lengths_and_what_lies_beyond_them(dev, T, lengths, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,H,Hk,Dk,Dv,lengths", [(4, 1210, 2, 1, 64, 64, [1210, 0, 1, 601]), (4, 530, 3, 3, 96, 64, [200, 530, 0, 385]),
+                                                    (3, 700, 16, 8, 72, 96, [700, 64, 333]), (2, 900, 1, 1, 128, 128, [899, 129])])
+def test_lengths_that_end_before_some_segments(dev, B, T, H, Hk, Dk, Dv, lengths, dtype):
+    """Long enough for segments of tokens, joined by the workgroups or by a scan, some of them without a token that counts."""
+    q, k, v, ld, s0, go, gs = inputs(dev, B, T, H, Hk, Dk, Dv, dtype, seed=T)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    want = mo.attention_grads(q, k, v, ld, Dk ** -0.5, go, gs, s0, lengths)
+    for b, m in enumerate(lengths):
+        for t in (q, k, v, go):
+            t[b, m:] = float("nan")
+    for t in (q, k, v, s0):
+        t.requires_grad_(True)
+    o, s = torch.ops.sffft.linear_attention(q, k, v, ld, Dk ** -0.5, s0, n)
+    got = (o, s, *torch.autograd.grad((o, s), (q, k, v, s0), (go, gs)))
+    for name, a, w in zip(("o", "state", "dq", "dk", "dv", "dstate"), got, want):
+        assert mo.rel_l2(a, w) < tol(a), (name, mo.rel_l2(a, w))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_extreme_decays(dev, dtype):
     """No memory at all (-inf), a decay that underflows within a chunk, none (0), and a slow one."""
     case = (2, 150, 4, 4, 64, 32)
