@@ -75,14 +75,15 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
                      dim3(256), 0, st, L);
   return hipGetLastError();
 }
-// Tiles of 64 or 128 channels. fp32 takes 64 of V: the planes of 128 leave no room for a second workgroup on a CU.
-// (bf16, two tiles of 64 of V instead of one of 128: 700 us against 570 for 131072 tokens.)
+// Tiles of 64 or 128 channels, of 96 for K (training, 8 x 12 heads of 96 and 600 tokens, bf16 and fp32: 83 and 207 us
+// instead of 94 and 230). fp32 takes 64 of V: the planes of 128 leave no room for a second workgroup on a CU. (bf16,
+// two tiles of 64 of V instead of one of 128: 700 us against 570 for 131072 tokens.)
 template <class T, class TO, bool OUT, int UP>
 hipError_t march_planes(la::Launch& L, hipStream_t st) {
   const int K = L.m[0].K, V = L.m[0].V;
   if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 2)
-    if (V > 64) return launch<T, TO, 128, 128, OUT, UP>(L, st);
+    if (V > 64) return K <= 96 ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 128, 128, OUT, UP>(L, st);
   if (K <= 96) return launch<T, TO, 96, 64, OUT, UP>(L, st);
   return launch<T, TO, 128, 64, OUT, UP>(L, st);
 }

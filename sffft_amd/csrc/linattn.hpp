@@ -268,7 +268,10 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   constexpr int NS = sizeof(T) == 4 ? 3 : 1, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, KA = KT / 16;
   constexpr int VW = VT / 64, TILES = MT * (MT + 1) / 2, NP = (TILES + 3) / 4;  // P's tiles, and those of a wavefront (some twice)
   constexpr int E = sizeof(TO);
-  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, KT + 16> ta;
+  constexpr int LK = KT == 96 ? 128 : KT;  // lanes that fetch K channels take these
+  // outputs leave through a's tile (below)
+  constexpr bool VIA = OUT && NS == 1 && E == 2 && LK == VT;
+  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, (VIA ? VT : KT) + 16> ta;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, KT + 16> tb;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, VT + 16> tc;
   __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, C + 8, false> tp;
@@ -305,7 +308,7 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   const int orow = L.s.H * m.V;
   TO* po = OUT ? static_cast<TO*>(m.out) + (((long long)b * L.s.T + t0) * L.s.H + h) * m.V : nullptr;
 
-  Stage<T, C, KT == 96 ? 128 : KT> ga, gb;
+  Stage<T, C, LK> ga, gb;
   Stage<T, C, VT> gc;
   auto fetch = [&](int n) {
     if constexpr (OUT) ga.load(pa, m.a.st, n, m.K);
@@ -402,7 +405,6 @@ __global__ __launch_bounds__(256, KT == 64 ? 3 : 2) void march_kernel(Launch L) 
   // by then, so that whole rows leave together (a store of 4 channels in each of 16 rows takes the
   // address unit 64 cycles, of 8 whole rows 16), each lane from the pieces that it will overwrite with the
   // next chunk's a; rows from `left` on are not written.
-  constexpr bool VIA = OUT && NS == 1 && E == 2 && KT == VT;
   f32x4 o[MT][VW] = {};
   int left = 0;
   auto stage_out = [&]() {
