@@ -75,12 +75,14 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
                      dim3(256), 0, st, L);
   return hipGetLastError();
 }
-// Tiles of 64 or 128 channels, of 96 for K (training, 8 x 12 heads of 96 and 600 tokens, bf16 and fp32: 83 and 207 us
-// instead of 94 and 230). fp32 takes 64 of V: the planes of 128 leave no room for a second workgroup on a CU. (bf16,
-// two tiles of 64 of V instead of one of 128: 700 us against 570 for 131072 tokens.)
+// Tiles of 32, 64, 96 or 128 channels of K, 64 or 128 of V. (In the next larger one instead, training, 8 x 12 heads
+// of 600 tokens, us: bf16 heads of 32 channels 51 for 45, of 96 94 for 83; fp32 95 for 68, 230 for 207.) fp32 takes
+// 64 of V: the planes of 128 leave no room for a second workgroup on a CU. (bf16, two tiles of 64 of V instead of one
+// of 128: 700 us against 570 for 131072 tokens.)
 template <class T, class TO, bool OUT, int UP>
 hipError_t march_planes(la::Launch& L, hipStream_t st) {
   const int K = L.m[0].K, V = L.m[0].V;
+  if (K <= 32) return launch<T, TO, 32, 64, OUT, UP>(L, st);
   if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 2)
     if (V > 64) return K <= 96 ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 128, 128, OUT, UP>(L, st);

@@ -87,6 +87,12 @@ def test_full_chip(dev, B, T, H, Hk, Dk, Dv, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,H,Hk,Dk,Dv", [(6, 1500, 12, 12, 32, 32), (3, 1800, 12, 4, 24, 96), (3, 1600, 12, 6, 72, 128), (3, 1700, 12, 12, 96, 64)])
+def test_full_chip_of_other_tiles(dev, B, T, H, Hk, Dk, Dv, dtype):
+    test_full_chip(dev, B, T, H, Hk, Dk, Dv, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("T,lengths", [(5, [0, 5, 1]), (130, [64, 0, 130]), (200, [199, 65, 63]), (64, [0, 0, 0])], ids=str)
 def test_lengths_and_what_lies_beyond_them(dev, T, lengths, dtype):
     """Tokens from lengths[b] on hold NaN and infinities: nothing of them reaches an output, their own are 0."""
