@@ -133,8 +133,10 @@ hipError_t forward(const sffft_linattn* p, const void* q, const void* k, const v
   const Cut cut = cut_of(p, 1);
   const March m = {operand(q, p->q, 1), operand(k, p->k, G), operand(v, p->v, G), o, s0, work, s1, p->Dk, p->Dv, p->Dv, 1,
                    0, p->scale, p->scale, 1.f};
-  la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1, cut.nseg > MAX_JOINED,
-                  cut.nseg > MAX_JOINED || (s1 && cut.nseg >= MIN_ALL)};
+  // A scan too where the last state takes the initial one's place: workgroups that join the segments read that one
+  // while another writes it.
+  const bool scanned = cut.nseg > MAX_JOINED || (cut.nseg > 1 && s1 && s1 == s0);
+  la::Launch L = {{m}, s, 1, cut.nseg, cut.seg, 1, scanned, scanned || (s1 && cut.nseg >= MIN_ALL)};
   hipError_t e = hipSuccess;
   if (cut.nseg > 1) e = march<T, false>(L, st);
   if (e == hipSuccess && L.scanned) {

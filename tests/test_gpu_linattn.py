@@ -331,6 +331,24 @@ def test_binding_matches_the_operators(dev):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("T", [1, 64, 130, 500, 1500])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_final_state_in_place_of_the_initial(dev, T, dtype):
+    """sffft_linattn_fwd may write the final state over the initial one, however many segments read that."""
+    B, H, D = 3, 12, 64
+    q, k, v, ld, s0, _, _ = inputs(dev, B, T, H, H, D, D, dtype, seed=T)
+    want = mixers.linear_attention(q, k, v, ld, 0.125, s0)
+    p = mixers.linattn_params(q, k, v, 0.125)
+    L, stream = mixers.lib(), torch.cuda.current_stream().cuda_stream
+    need = L.sffft_linattn_work_bytes(p, 0)
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    for _ in range(4):
+        s, o = s0.clone(), torch.empty_like(want[0])
+        assert L.sffft_linattn_fwd(p, q.data_ptr(), k.data_ptr(), v.data_ptr(), ld.data_ptr(), s.data_ptr(), None, o.data_ptr(),
+                                   s.data_ptr(), work.data_ptr(), work.numel(), stream) == 0
+        assert mo.rel_l2(s, want[1].cpu()) < FP32 and mo.rel_l2(o, want[0].cpu()) < tol(o)
+
+
 def test_state_beyond_two_gib(dev):
     """A state cache whose offsets pass 32 bits: the last slot is the one used."""
     H, D = 16, 128
