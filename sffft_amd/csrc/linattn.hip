@@ -53,7 +53,7 @@ struct Cut {
 };
 Cut cut_of(const sffft_linattn* p, int marches) {
   const int C = p->io ? la::chunk_of<uint16_t>() : la::chunk_of<float>(), D = std::max(p->Dk, p->Dv);
-  const int chunks = (p->T + C - 1) / C, fill = D > 64 ? 512 : 1024;
+  const int chunks = (p->T - 1) / C + 1, fill = D > 64 ? 512 : 1024;
   const long long heads = (long long)p->B * p->H * marches;
   const int want = (int)std::min<long long>(chunks, std::max<long long>(1, fill / heads));
   const int few = (chunks + MAX_JOINED - 1) / MAX_JOINED, joined = (chunks + few - 1) / few;

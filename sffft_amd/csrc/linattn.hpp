@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256, KT <= 64 ? 3 : 2) void march_kernel(Launch L) 
   const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool rev = m.rev;
-  const int first = z * L.seg, last = min(first + L.seg, L.s.T), chunks = (last - first + C - 1) / C;
+  const int first = z * L.seg, last = first + min(L.seg, L.s.T - first), chunks = (last - first + C - 1) / C;
   const int end = min(valid_tokens(L.s, b), last);  // of the tokens that count
   const float l2 = decay_log2(L.s.log_decay, h);
   auto power = [&](int n) { return n < 0 ? 0.f : __builtin_amdgcn_exp2f(l2 * (float)n); };
