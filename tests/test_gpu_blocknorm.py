@@ -176,6 +176,25 @@ def test_rows_between_boundaries(dev, B, T, C, gate, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T,C", [(700, 1531), (9000, 100), (9000, 37), (30, 2047)])
+def test_odd_rows_within_wider_ones(dev, T, C, dtype):
+    """Columns of wider arrays, NaN beside them: rows that start at the same distance from a boundary as the outputs', and others."""
+    t, gr, gh = inputs(dev, (1, T, C), dtype, "token", seed=C)
+    want, wgrads = oracle(t, "silu", gr, gh)
+
+    def within(x, more, at):
+        wide = torch.full((1, T, C + more), float("nan"), dtype=dtype, device=dev)
+        wide[..., at:at + C] = x
+        return wide[..., at:at + C]
+
+    for more, at in ((16, 0), (8, 8), (5, 2)):
+        m = dict(t, **{n: within(t[n], more, at) for n in ("x", "y", "gate")})
+        out, grads = run(m, "silu", within(gr, more, at), within(gh, more, at))
+        for name, a, w in zip(("r", "h") + NAMES, (*out, *grads), (*want, *wgrads)):
+            assert mo.rel_l2(a, w) < tol(a), (more, at, name, mo.rel_l2(a, w))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("gate", ["token", "sequence", "none"])
 @pytest.mark.parametrize("B,T,C", [(1, 1, 2), (5, 3, 8), (2, 77, 37), (3, 41, 64), (2, 5, 100), (1, 1001, 121), (2, 333, 128), (3, 35, 129),
                                    (1, 9, 200), (2, 50, 249), (1, 70, 256), (2, 70000, 64)])
