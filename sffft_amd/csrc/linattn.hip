@@ -77,16 +77,20 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
 }
 // Tiles of 32, 64, 96 or 128 channels of K, 64 or 128 of V. (In the next larger one instead, training, 8 x 12 heads
 // of 600 tokens, us: bf16 heads of 32 channels 51 for 45, of 96 94 for 83; fp32 95 for 68, 230 for 207.) fp32 takes
-// 64 of V: the planes of 128 leave no room for a second workgroup on a CU. (bf16, two tiles of 64 of V instead of one
-// of 128: 700 us against 570 for 131072 tokens.)
+// 128 of V up to 96 of K: the planes of more leave no room for a second workgroup on a CU (two tiles of 64 of V
+// instead: 170 us for 151 at 64 x 96 channels, 209 for 178 at 96 x 96). bf16 takes two tiles of 64 of V beside 64 of
+// K, whose outputs leave as whole rows (one of 128: 0.89 to 1.10 times as fast), and one of 128 beside more (two: 700
+// us against 570 for 131072 tokens).
 template <class T, class TO, bool OUT, int UP>
 hipError_t march_planes(la::Launch& L, hipStream_t st) {
   const int K = L.m[0].K, V = L.m[0].V;
   if (K <= 32) return launch<T, TO, 32, 64, OUT, UP>(L, st);
+  if constexpr (sizeof(T) == 4)
+    if (K <= 64 && V > 64) return launch<T, TO, 64, 128, OUT, UP>(L, st);
   if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
+  if (K <= 96) return V > 64 ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 96, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 2)
-    if (V > 64) return K <= 96 ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 128, 128, OUT, UP>(L, st);
-  if (K <= 96) return launch<T, TO, 96, 64, OUT, UP>(L, st);
+    if (V > 64) return launch<T, TO, 128, 128, OUT, UP>(L, st);
   return launch<T, TO, 128, 64, OUT, UP>(L, st);
 }
 // nm marches of the same K and V

@@ -264,7 +264,7 @@ constexpr int chunk_of() { return sizeof(T) == 4 ? 32 : 64; }
 // The next chunk is fetched a chunk ahead, and a chunk's outputs leave at the start of the next, before that
 // fetch: the wait for it then finds them gone.
 template <class T, class TO, int KT, int VT, bool OUT, int UP>
-__global__ __launch_bounds__(256, KT <= 64 ? 3 : 2) void march_kernel(Launch L) {
+__global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kernel(Launch L) {
   constexpr int NS = sizeof(T) == 4 ? 3 : 1, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, KA = KT / 16;
   constexpr int VW = VT / 64, TILES = MT * (MT + 1) / 2, NP = (TILES + 3) / 4;  // P's tiles, and those of a wavefront (some twice)
   constexpr int E = sizeof(TO);
