@@ -14,12 +14,12 @@
 // segment's own state, and the march starts every segment with the decayed sums of those before it, which it joins
 // itself or, where they are many, finds joined by a scan.
 //
-// Operands in 16 bits: bf16 inputs are exact; P and the entering state are rounded to bf16 where they are operands of
-// a product that is rounded to bf16 itself in the end (their errors are of that rounding's size). The state is fp32
-// and so are the decayed c_j that are added to it: they are split into three bf16 parts (8 bits each, 24 together),
-// one product each; into two where the state only serves outputs of 16 bits. fp32 inputs are split so too, and every
-// product of two split operands is the six partial products above 2^-24 (a bf16 product at 1240 TFLOP/s, an fp32 one
-// at 154).
+// Operands in 16 bits: bf16 inputs are exact. P and the entering state, operands of products that are rounded to bf16
+// in the end, are split into two bf16 parts (17 bits: 2^-9 of that rounding), one product each; in one part each they
+// made the outputs' error 2.3e-3 where their own rounding is 1.7e-3. The state is fp32 and so are the decayed c_j that
+// are added to it: they are split into three bf16 parts (8 bits each, 24 together), into two where the state only
+// serves outputs of 16 bits. fp32 inputs are split so too, and every product of two split operands is the six
+// partial products above 2^-24 (a bf16 product at 1240 TFLOP/s, an fp32 one at 154).
 //
 // Measured (bf16, us): 131072 tokens, 12 heads of 128: 549, sums 160 and march 368 at 4.5 TB/s, bound by memory (k
 // and v are read twice); training, 8 x 2048 tokens, 12 heads of 64: 114, sums 13 and 18, march 25 forward and 58 for
@@ -167,10 +167,13 @@ struct Tile {
   static __device__ __forceinline__ int at(int row, int col) { return SWAP ? col ^ (row & 8) : col; }
 
   // operand whose index is the row: lane (g, i) holds channels at..at+7 of row r0 + i, at = c0 + 8 g
+  __device__ __forceinline__ bf16x8 plane(int p, int r0, int c0, int i, int g) const {
+    return *reinterpret_cast<const bf16x8*>(&v[p][r0 + i][c0 + at(i, 8 * g)]);
+  }
   __device__ __forceinline__ Frag<NS> rows(int r0, int c0, int i, int g) const {
     Frag<NS> f;
 #pragma unroll
-    for (int p = 0; p < NS; p++) f.p[p] = *reinterpret_cast<const bf16x8*>(&v[p][r0 + i][c0 + at(i, 8 * g)]);
+    for (int p = 0; p < NS; p++) f.p[p] = plane(p, r0, c0, i, g);
     return f;
   }
   // the same with the channels in the order of an accumulator's rows: c0 + 4 g .. + 3 and c0 + 16 + 4 g .. + 3
@@ -265,7 +268,7 @@ constexpr int chunk_of() { return sizeof(T) == 4 ? 32 : 64; }
 // fetch: the wait for it then finds them gone.
 template <class T, class TO, int KT, int VT, bool OUT, int UP>
 __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kernel(Launch L) {
-  constexpr int NS = sizeof(T) == 4 ? 3 : 1, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, KA = KT / 16;
+  constexpr int NS = sizeof(T) == 4 ? 3 : 1, PX = sizeof(T) == 4 ? 3 : 2, C = chunk_of<T>(), MT = C / 16, JS = C / 32, KS = KT / 32, KA = KT / 16;
   constexpr int VW = VT / 64, TILES = MT * (MT + 1) / 2, NP = (TILES + 3) / 4;  // P's tiles, and those of a wavefront (some twice)
   constexpr int E = sizeof(TO);
   constexpr int LK = KT == 96 ? 128 : KT;  // lanes that fetch K channels take these
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, (VIA ? VT : KT) + 16> ta;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, KT + 16> tb;
   __shared__ __attribute__((aligned(16))) Tile<NS, C, VT + 16> tc;
-  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, C + 8, false> tp;
+  __shared__ __attribute__((aligned(16))) Tile<PX, OUT ? C : 1, C + 8, false> tp;  // PX: planes of P and X
   __shared__ __attribute__((aligned(16))) float fi[C], wj[C];  // decays: of the entering state at row i, of token j in the update
 
   // Workgroups go to the 8 XCDs in turn; the marches and V tiles of one head and segment, which read the same
@@ -488,8 +491,12 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
         // stored in the order of the transposing reads' rows: 16 * (j / 16 % 2) + 4 g + e at 8 g + 4 (j / 16 % 2) + e
         u16* q = &tp.v[0][16 * pi[t] + i16][32 * (pj[t] >> 1) + 8 * g + 4 * (pj[t] & 1)];
         const float x0 = d[0] * pd[t][0], x1 = d[1] * pd[t][1], x2 = d[2] * pd[t][2], x3 = d[3] * pd[t][3];
-        if constexpr (NS == 1) {
-          *reinterpret_cast<uint2*>(q) = make_uint2(ops::pack_bf16(x0, x1), ops::pack_bf16(x2, x3));
+        if constexpr (PX == 2) {
+          uint2 hh, mm;
+          split2(x0, x1, hh.x, mm.x);
+          split2(x2, x3, hh.y, mm.y);
+          *reinterpret_cast<uint2*>(q) = hh;
+          *reinterpret_cast<uint2*>(q + C * (C + 8)) = mm;
         } else {
           uint2 hh, mm, ll;
           split2(x0, x1, hh.x, mm.x, ll.x);
@@ -506,7 +513,8 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
         for (int v = 0; v < VW; v++) o[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        Frag<NS> fs[VW], fa[MT];
+        Frag<PX> fs[VW];
+        Frag<NS> fa[MT];
 #pragma unroll
         for (int t = 0; t < MT; t++) fa[t] = ta.rows_acc(16 * t, 32 * k, i16, g);
 #pragma unroll
@@ -514,9 +522,9 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; e++) x[e] = S[2 * k + (e >> 2)][v][e & 3];
-          fs[v] = split8<NS>(x);
+          fs[v] = split8<PX>(x);
         }
-        products<NS, NS, MT * VW>([&](int n) -> auto& { return fs[n % VW]; }, [&](int n) -> auto& { return fa[n / VW]; },
+        products<PX, NS, MT * VW>([&](int n) -> auto& { return fs[n % VW]; }, [&](int n) -> auto& { return fa[n / VW]; },
                                   [&](int n) -> auto& { return o[n / VW][n % VW]; });
       }
 #pragma unroll
@@ -553,11 +561,19 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
         fw[v] = split8<UP>(x);
       }
       if constexpr (OUT) {
-        Frag<NS> fp[MT];  // the zero tiles too: their two products cost less than branches
+        // the zero tiles too: their two products cost less than branches. Where there is one plane of c, P's come one
+        // by one, for their registers.
+        constexpr int AT_ONCE = NS == 1 ? 1 : PX;
 #pragma unroll
-        for (int t = 0; t < MT; t++) fp[t] = tp.rows(16 * t, 32 * s, i16, g);
-        products<NS, NS, MT * VW>([&](int n) -> auto& { return fc[n % VW]; }, [&](int n) -> auto& { return fp[n / VW]; },
-                                  [&](int n) -> auto& { return o[n / VW][n % VW]; });
+        for (int p = PX - AT_ONCE; p >= 0; p -= AT_ONCE) {
+          Frag<AT_ONCE> fp[MT];
+#pragma unroll
+          for (int t = 0; t < MT; t++)
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) fp[t].p[k] = tp.plane(p + k, 16 * t, 32 * s, i16, g);
+          products<NS, AT_ONCE, MT * VW>([&](int n) -> auto& { return fc[n % VW]; }, [&](int n) -> auto& { return fp[n / VW]; },
+                                         [&](int n) -> auto& { return o[n / VW][n % VW]; });
+        }
       }
       constexpr int HALF = 2;
 #pragma unroll
