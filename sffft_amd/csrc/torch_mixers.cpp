@@ -439,8 +439,18 @@ bool recorded(const A&... t) {
   return at::GradMode::is_enabled() && (wants_grad(t) || ...);
 }
 
-void refuse_second_derivative(const char* op) {
+// No operator has a forward-mode derivative. A tangent needs no requires_grad and no recording: a call below autograd
+// would drop it, and its output's would read as zero.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+template <class... A>
+void refuse_tangents(const char* op, const A&... t) {
+  TORCH_CHECK(!(has_tangent(t) || ...), op, " has no forward-mode derivative (jvp)");
+}
+
+void refuse_second_derivative(const char* op, const variable_list& grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, " has no second derivative (backward with create_graph)");
+  for (const Variable& g : grads) refuse_tangents(op, g);
 }
 
 class AttentionFn : public torch::autograd::Function<AttentionFn> {
@@ -457,7 +467,7 @@ class AttentionFn : public torch::autograd::Function<AttentionFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = op_handle<AttentionBackwardSig>("sffft::linear_attention_backward");
-    refuse_second_derivative(LA);
+    refuse_second_derivative(LA, grads);
     const variable_list s = ctx->get_saved_variables();
     variable_list out(7);
     if (!grads[0].defined() && !grads[1].defined()) return out;
@@ -474,6 +484,7 @@ std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& k, 
                                               const OptTensor& lengths) {
   TORCH_CHECK(!log_decay.requires_grad() || !at::GradMode::is_enabled(), LA,
               ": log_decay has no gradient (the decays are constants of the layer)");
+  refuse_tangents(LA, q, k, v, log_decay, state);
   if (!recorded(q, k, v, state)) {
     static const auto op = op_handle<AttentionSig>("sffft::linear_attention");
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -488,6 +499,7 @@ Tensor step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   static const auto op = op_handle<StepSig>("sffft::linear_attention_step");
   TORCH_CHECK(!recorded(q, k, v, state, log_decay),
               "sffft::linear_attention_step has no gradient: use sffft::linear_attention");
+  refuse_tangents("sffft::linear_attention_step", q, k, v, log_decay, state);
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor o = op.call(q, k, v, log_decay, state, scale, slots);
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
@@ -522,6 +534,7 @@ class RotaryFn : public torch::autograd::Function<RotaryFn> {
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& table,
                                            const OptTensor& positions, bool interleaved, bool inverse) {
   TORCH_CHECK(!table.requires_grad() || !at::GradMode::is_enabled(), ROT, ": the table has no gradient");
+  refuse_tangents(ROT, q, k, table);
   if (!recorded(q, k)) {
     static const auto op = op_handle<RotarySig>("sffft::rotary");
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -536,6 +549,7 @@ void rotary_inplace_autograd(const Tensor& q, const Tensor& k, const Tensor& tab
   static const auto op = op_handle<RotaryInplaceSig>("sffft::rotary_");
   TORCH_CHECK(!recorded(q, k),
               "sffft::rotary_ records no gradient: use sffft::rotary");
+  refuse_tangents("sffft::rotary_", q, k, table);
   at::AutoDispatchBelowADInplaceOrView guard;
   op.call(q, k, table, positions, interleaved);
   for (const Tensor* t : {&q, &k})
@@ -558,7 +572,7 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = op_handle<NormBackwardSig>("sffft::block_norm_backward");
-    refuse_second_derivative(BN);
+    refuse_second_derivative(BN, grads);
     const variable_list s = ctx->get_saved_variables();
     variable_list out(8);
     if (!grads[0].defined() && !grads[1].defined()) return out;
@@ -575,6 +589,7 @@ class BlockNormFn : public torch::autograd::Function<BlockNormFn> {
 std::tuple<Tensor, Tensor> block_norm_autograd(const Tensor& x, const Tensor& y, const Tensor& w_pre,
                                                const OptTensor& w_post, const OptTensor& gate, const OptTensor& scale,
                                                c10::string_view activation, double eps) {
+  refuse_tangents(BN, x, y, w_pre, w_post, gate, scale);
   if (!recorded(x, y, w_pre, w_post, gate, scale)) {
     static const auto op = op_handle<BlockNormSig>("sffft::block_norm");
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -595,7 +610,7 @@ class PreNormFn : public torch::autograd::Function<PreNormFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = op_handle<NormBackwardSig>("sffft::block_norm_backward");
-    refuse_second_derivative("sffft::pre_norm");
+    refuse_second_derivative("sffft::pre_norm", grads);
     const variable_list s = ctx->get_saved_variables();
     auto g = op.call(std::nullopt, grads[0], s[0], std::nullopt, s[1], std::nullopt, std::nullopt, std::nullopt, "none",
                      ctx->saved_data["eps"].toDouble());
@@ -604,6 +619,7 @@ class PreNormFn : public torch::autograd::Function<PreNormFn> {
 };
 
 Tensor pre_norm_autograd(const Tensor& x, const Tensor& w, double eps) {
+  refuse_tangents("sffft::pre_norm", x, w);
   if (!recorded(x, w)) {
     static const auto op = op_handle<PreNormSig>("sffft::pre_norm");
     at::AutoDispatchBelowADInplaceOrView guard;
