@@ -239,13 +239,16 @@ void rotary_run(const Tensor& q, const Tensor& k, const Tensor& table_in, const 
                 pos->sizes());
     p.pos_bits = pos->scalar_type() == at::kLong ? 64 : 32;
   }
-  if (B * T * q.size(2) == 0) return;
+  if (B * T * (q.size(2) + k.size(2)) == 0) return;
   const Tensor table = table_in.contiguous();
-  p.B = (int)B, p.T = (int)T, p.H = (int)q.size(2), p.Hk = (int)k.size(2), p.D = (int)q.size(3);
+  // the call's first array has heads: k's where q has none
+  const bool alone = q.size(2) == 0;
+  const Tensor &a = alone ? k : q, &c = alone ? q : k, &ao = alone ? ko : qo, &co = alone ? qo : ko;
+  p.B = (int)B, p.T = (int)T, p.H = (int)a.size(2), p.Hk = (int)c.size(2), p.D = (int)a.size(3);
   p.R = (int)table.size(1), p.interleaved = interleaved, p.inverse = inverse, p.positions = (int)table.size(0);
-  for (int i = 0; i < 3; i++) p.q[i] = q.stride(i), p.k[i] = k.stride(i), p.qo[i] = qo.stride(i), p.ko[i] = ko.stride(i);
-  check(sffft_rotary_apply(&p, ptr(q), ptr(k), table.const_data_ptr<float>(), ptr(pos), qo.data_ptr(),
-                           p.Hk ? ko.data_ptr() : nullptr, stream_of()),
+  for (int i = 0; i < 3; i++) p.q[i] = a.stride(i), p.k[i] = c.stride(i), p.qo[i] = ao.stride(i), p.ko[i] = co.stride(i);
+  check(sffft_rotary_apply(&p, ptr(a), ptr(c), table.const_data_ptr<float>(), ptr(pos), ao.data_ptr(),
+                           p.Hk ? co.data_ptr() : nullptr, stream_of()),
         ROT);
 }
 
