@@ -171,7 +171,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_gpu(
                 ": the final state's gradient must be [B, H, Dk, Dv], got ", ds_in->sizes());
   }
   const OptTensor ds = dense(ds_in);
-  if (B == 0 || H == 0) return {dq, dk, dv, ds0};
+  if (B == 0 || H == 0) return {dq, dk.zero_(), dv.zero_(), ds0};  // keys without queries
   if (T == 0) {
     if (a.state && ds) ds0.copy_(*ds);
     else ds0.zero_();

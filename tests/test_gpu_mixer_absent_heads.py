@@ -32,3 +32,16 @@ def test_rotary_of_keys_alone(dev, interleaved, dtype):
     torch.ops.sffft.rotary_(none, y, table, None, interleaved)
     assert torch.equal(y, want)
     assert mo.rel_l2(got, mo.rotary(k, table, None, interleaved)) < (2.0 ** -8 if dtype == torch.bfloat16 else 1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_attention_without_queries(dev, dtype):
+    """Nothing depends on the keys and values: their gradients are zero."""
+    k, v = (torch.randn(2, 9, 3, 64).to(dtype).to(dev).requires_grad_() for _ in range(2))
+    q, s0 = torch.zeros(2, 9, 0, 64, dtype=dtype, device=dev), torch.zeros(2, 0, 64, 64, device=dev).requires_grad_()
+    leave_marks(dev, k.shape)
+    o, s = torch.ops.sffft.linear_attention(q, k, v, torch.zeros(0, device=dev), 0.1, s0)
+    assert o.shape == (2, 9, 0, 64) and s.shape == (2, 0, 64, 64)
+    leave_marks(dev, k.shape)
+    for g, x in zip(torch.autograd.grad((o, s), (k, v, s0), (torch.zeros_like(o), torch.zeros_like(s))), (k, v, s0)):
+        assert torch.equal(g, torch.zeros_like(x))
