@@ -11,6 +11,8 @@
  *  - `stream` is a hipStream_t (NULL = default stream). Calls are asynchronous on that stream,
  *    allocate nothing, keep nothing between calls, and may be captured, the first one too.
  *  - Outputs and workspace may overlap no input, unless a call says otherwise.
+ *  - Sizes whose kernels would need 2^32 threads are refused (attention: B * H from 2^24 / 6 on in the
+ *    backward pass at the least, 2^23 forward, 2^24 for single tokens; norms: 2^19 gates that rows share).
  *  - Sums, states and statistics are fp32; every sum has a fixed order (no atomics), so equal
  *    calls give equal bits.
  */

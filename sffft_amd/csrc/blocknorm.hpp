@@ -484,51 +484,54 @@ __global__ __launch_bounds__(BLK < 64 ? 64 : BLK) void bwd_kernel(Args A) {
 
 // The sums of the parts (37 MB, 1024 parts of three quantities of 1531 channels: 7 us). Workgroups take 32 columns of
 // one quantity: the nparts parts of dwq and of t, which gives dwp and ds, then for each gate that rows share its
-// `per` consecutive parts.
+// `per` consecutive parts. There may be more quantities than the grid has rows.
 struct SumArgs {
   const float *parts, *wp, *sc;
   float *dwq, *dwp, *ds;
   void* dgate;
   int C, bf16, y;
-  long long nparts, per;
+  long long nparts, per, sums;
 };
 __global__ __launch_bounds__(1024) void sum_kernel(SumArgs A) {
   __shared__ float lds[32][33];
-  const int tiles = (A.C + 31) / 32, which = blockIdx.x / tiles, lc = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int c = (blockIdx.x - which * tiles) * 32 + lc;
-  // which: 0 = dwq, 1 = t (where there is a y), then the gates
-  const int gate = which - (A.y ? 2 : 1);
-  const long long n = gate < 0 ? A.nparts : A.per, at = gate < 0 ? which * A.nparts : 2 * A.nparts + gate * A.per;
-  const float* p = A.parts + at * A.C + c;
-  float s = 0.f;
-  if (c < A.C) {
-    long long i = g;
-    for (; i + 7 * 32 < n; i += 8 * 32) {
-      float v[8];
+  const int lc = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + lc;
+  for (long long which = blockIdx.y; which < A.sums; which += gridDim.y) {
+    // which: 0 = dwq, 1 = t (where there is a y), then the gates
+    const long long gate = which - (A.y ? 2 : 1);
+    const long long n = gate < 0 ? A.nparts : A.per, at = gate < 0 ? which * A.nparts : 2 * A.nparts + gate * A.per;
+    const float* p = A.parts + at * A.C + c;
+    float s = 0.f;
+    if (c < A.C) {
+      long long i = g;
+      for (; i + 7 * 32 < n; i += 8 * 32) {
+        float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = p[(i + 32 * k) * A.C];
+        for (int k = 0; k < 8; k++) v[k] = p[(i + 32 * k) * A.C];
 #pragma unroll
-      for (int k = 0; k < 8; k++) s += v[k];
+        for (int k = 0; k < 8; k++) s += v[k];
+      }
+      for (; i < n; i += 32) s += p[i * A.C];
     }
-    for (; i < n; i += 32) s += p[i * A.C];
-  }
-  lds[g][lc] = s;
-  ops::barrier();
-  // 32 lanes add 32 rows: lane (g, lc) of the first wavefronts takes column g
-  s = lds[lc][g];
+    lds[g][lc] = s;
+    ops::barrier();
+    // 32 lanes add 32 rows: lane (g, lc) of the first wavefronts takes column g
+    s = lds[lc][g];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor(s, o);
-  const int col = (blockIdx.x - which * tiles) * 32 + g;
-  if (lc || col >= A.C) return;
-  if (which == 0) {
-    A.dwq[col] = s;
-  } else if (gate < 0) {
-    if (A.dwp) A.dwp[col] = A.sc ? A.sc[col] * s : s;
-    if (A.ds) A.ds[col] = A.wp ? A.wp[col] * s : s;
-  } else if (A.bf16) {
-    ops::put(static_cast<uint16_t*>(A.dgate) + (long long)gate * A.C + col, s);
-  } else {
-    static_cast<float*>(A.dgate)[(long long)gate * A.C + col] = s;
+    for (int o = 16; o; o >>= 1) s += __shfl_xor(s, o);
+    const int col = blockIdx.x * 32 + g;
+    if (!lc && col < A.C) {
+      if (which == 0) {
+        A.dwq[col] = s;
+      } else if (gate < 0) {
+        if (A.dwp) A.dwp[col] = A.sc ? A.sc[col] * s : s;
+        if (A.ds) A.ds[col] = A.wp ? A.wp[col] * s : s;
+      } else if (A.bf16) {
+        ops::put(static_cast<uint16_t*>(A.dgate) + gate * A.C + col, s);
+      } else {
+        static_cast<float*>(A.dgate)[gate * A.C + col] = s;
+      }
+    }
+    ops::barrier();  // before the next sum takes the array
   }
 }
 

@@ -66,12 +66,14 @@ Cut cut_of(const sffft_linattn* p, int marches) {
 // for three marches also where each has a launch of its own: the fp32 step above 196 us instead of 162.)
 int backward_marches(const sffft_linattn* p) { return p->Dk == p->Dv && (p->H == p->Hk || !p->io) ? 3 : 1; }
 
+// Workgroups of nm marches over units of a head and a segment.
+long long workgroups(long long units, int nm, int vtiles) { return (units + 7) / 8 * 8 * nm * vtiles; }
+
 template <class T, class TO, int KT, int VT, bool OUT, int UP>
 hipError_t launch(la::Launch& L, hipStream_t st) {
-  L.vtiles = 1;
-  for (int i = 0; i < L.nm; i++) L.vtiles = std::max(L.vtiles, (L.m[i].V + VT - 1) / VT);
+  L.vtiles = (L.m[0].V + VT - 1) / VT;
   const int units = L.s.B * L.s.H * (OUT || L.all ? L.nseg : L.nseg - 1);
-  hipLaunchKernelGGL((la::march_kernel<T, TO, KT, VT, OUT, UP>), dim3((unsigned)((units + 7) / 8 * 8 * L.nm * L.vtiles)),
+  hipLaunchKernelGGL((la::march_kernel<T, TO, KT, VT, OUT, UP>), dim3((unsigned)workgroups(units, L.nm, L.vtiles)),
                      dim3(256), 0, st, L);
   return hipGetLastError();
 }
@@ -81,16 +83,21 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
 // instead: 170 us for 151 at 64 x 96 channels, 209 for 178 at 96 x 96). bf16 takes two tiles of 64 of V beside 64 of
 // K, whose outputs leave as whole rows (one of 128: 0.89 to 1.10 times as fast), and one of 128 beside more (two: 700
 // us against 570 for 131072 tokens).
+int v_tile(int elem, int K, int V) {
+  const bool wide = elem == 4 ? K > 32 && K <= 96 : K > 64;
+  return V > 64 && wide ? 128 : 64;
+}
 template <class T, class TO, bool OUT, int UP>
 hipError_t march_planes(la::Launch& L, hipStream_t st) {
-  const int K = L.m[0].K, V = L.m[0].V;
+  const int K = L.m[0].K;
+  const bool wide = v_tile(sizeof(T), K, L.m[0].V) == 128;
   if (K <= 32) return launch<T, TO, 32, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 4)
-    if (K <= 64 && V > 64) return launch<T, TO, 64, 128, OUT, UP>(L, st);
+    if (K <= 64 && wide) return launch<T, TO, 64, 128, OUT, UP>(L, st);
   if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
-  if (K <= 96) return V > 64 ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 96, 64, OUT, UP>(L, st);
+  if (K <= 96) return wide ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 96, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 2)
-    if (V > 64) return launch<T, TO, 128, 128, OUT, UP>(L, st);
+    if (wide) return launch<T, TO, 128, 128, OUT, UP>(L, st);
   return launch<T, TO, 128, 64, OUT, UP>(L, st);
 }
 // nm marches of the same K and V
@@ -108,12 +115,11 @@ hipError_t scan(const la::ScanLaunch& L, int n, hipStream_t st) {
   return hipGetLastError();
 }
 
+long long head_sum_workgroups(long long n) { return (n / 4 + 255) / 256; }
 template <class T>
 hipError_t head_sums(la::HeadSums L, hipStream_t st) {
-  unsigned blocks[2];
-  for (int i = 0; i < 2; i++) blocks[i] = (unsigned)((L.s[i].n / 4 + 255) / 256);
-  L.blocks = blocks[0];
-  hipLaunchKernelGGL(la::head_sum_kernel<T>, dim3(blocks[0] + blocks[1]), dim3(256), 0, st, L);
+  L.blocks = (unsigned)head_sum_workgroups(L.s[0].n);
+  hipLaunchKernelGGL(la::head_sum_kernel<T>, dim3(L.blocks + (unsigned)head_sum_workgroups(L.s[1].n)), dim3(256), 0, st, L);
   return hipGetLastError();
 }
 
@@ -128,6 +134,24 @@ constexpr int MIN_ALL = 4;
 // dk and dv of heads that are shared, for each query head, before their sum
 size_t shared_bytes(const sffft_linattn* p) {
   return p->H == p->Hk ? 0 : (size_t)p->B * p->T * p->H * (p->Dk + p->Dv) * 4;
+}
+
+// Arguments that fit every launch of a forward or backward call, the largest of each size of marches.
+bool valid_call(const sffft_linattn* p, int backward) {
+  if (!valid_shape(p)) return false;
+  const int nseg = cut_of(p, backward ? backward_marches(p) : 1).nseg, elem = p->io ? 2 : 4;
+  const auto fits = [&](int nm, int K, int V) {
+    const int VT = v_tile(elem, K, V);
+    return ops::launchable(workgroups((long long)p->B * p->H * nseg, nm, (V + VT - 1) / VT), 256);
+  };
+  if (!backward) return fits(1, p->Dk, p->Dv);
+  const long long tokens = (long long)p->B * p->T;
+  const bool parts = p->H != p->Hk;
+  if (parts && !ops::launchable(head_sum_workgroups(tokens * p->Hk * p->Dk) + head_sum_workgroups(tokens * p->Hk * p->Dv), 256))
+    return false;
+  const int together = parts && p->io ? 1 : 2;  // marches that share a launch where Dk and Dv differ
+  return p->Dk == p->Dv ? fits(together + 1, p->Dk, p->Dv)
+                        : fits(nseg > 1 ? 2 : 1, p->Dk, p->Dv) && fits(together, p->Dv, p->Dk);
 }
 
 template <class T>
@@ -198,7 +222,7 @@ using namespace sffft;
 extern "C" {
 
 size_t sffft_linattn_work_bytes(const sffft_linattn* p, int backward) {
-  if (!valid_shape(p)) return 0;
+  if (!valid_call(p, backward)) return 0;
   return backward ? 2 * state_bytes(p, cut_of(p, backward_marches(p))) + shared_bytes(p) : state_bytes(p, cut_of(p, 1));
 }
 
@@ -206,7 +230,7 @@ int sffft_linattn_fwd(const sffft_linattn* p, const void* q, const void* k, cons
                       const float* initial_state, const int* lengths, void* o, float* final_state, void* work,
                       size_t work_bytes, void* stream) {
   size_t nq, nk, nv;
-  if (!valid_shape(p) || !log_decay || !o || !ops::aligned(o, 16) || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
+  if (!valid_call(p, 0) || !log_decay || !o || !ops::aligned(o, 16) || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
       !valid_input(k, p->k, p, p->Hk, p->Dk, &nk) || !valid_input(v, p->v, p, p->Hk, p->Dv, &nv) ||
       !ops::aligned(initial_state, 16) || !ops::aligned(final_state, 16) || !ops::aligned(log_decay, 4) ||
       !ops::aligned(lengths, 4))
@@ -235,7 +259,7 @@ int sffft_linattn_bwd(const sffft_linattn* p, const void* q, const void* k, cons
                       void* dq, void* dk, void* dv, float* d_initial_state, void* work, size_t work_bytes,
                       void* stream) {
   size_t nq, nk, nv, no;
-  if (!valid_shape(p) || !log_decay || !dq || !dk || !dv || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
+  if (!valid_call(p, 1) || !log_decay || !dq || !dk || !dv || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
       !valid_input(k, p->k, p, p->Hk, p->Dk, &nk) || !valid_input(v, p->v, p, p->Hk, p->Dv, &nv) ||
       !valid_input(go, p->go, p, p->H, p->Dv, &no) || !ops::aligned(initial_state, 16) ||
       !ops::aligned(d_final_state, 16) || !ops::aligned(d_initial_state, 16) || !ops::aligned(dq, 16) ||
@@ -264,7 +288,7 @@ int sffft_linattn_bwd(const sffft_linattn* p, const void* q, const void* k, cons
 int sffft_linattn_step(const sffft_linattn* p, const void* q, const void* k, const void* v, const float* log_decay,
                        float* state, int slots, const int* slot, void* o, void* stream) {
   size_t nq, nk, nv;
-  if (!valid_shape(p) || p->T != 1 || !log_decay || !state || !o || slots < 1 || !ops::aligned(state, 16) ||
+  if (!valid_shape(p) || p->T != 1 || !ops::launchable((long long)p->B * p->H, 256) || !log_decay || !state || !o || slots < 1 || !ops::aligned(state, 16) ||
       !ops::aligned(o, 16) || !valid_input(q, p->q, p, p->H, p->Dk, &nq) ||
       !valid_input(k, p->k, p, p->Hk, p->Dk, &nk) || !valid_input(v, p->v, p, p->Hk, p->Dv, &nv) ||
       !ops::aligned(log_decay, 4) || !ops::aligned(slot, 4))

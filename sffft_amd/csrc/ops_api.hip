@@ -29,14 +29,20 @@ namespace {
 
 // Vectors of 16 bytes where everything is aligned to them, else channel by channel (the two workloads of rotary.hpp:
 // 137 us against 277, 59 against 148 for two calls). About one unit for each of a workgroup's 256 lanes.
-template <class T>
-hipError_t rotary(rot::Args a, bool interleaved, bool wide, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const int pp = !wide ? 1 : interleaved ? V / 2 : V;
+bool rotary_grid(rot::Args& a, int elem, bool interleaved, bool wide) {
+  const int V = 16 / elem, pp = !wide ? 1 : interleaved ? V / 2 : V;
   a.units = a.D / (2 * pp), a.per = a.heads * a.units;
   const auto inverse = [](unsigned d) { return (unsigned)((((unsigned long long)1 << 32) + d - 1) / d); };
   a.by_units = inverse(a.units), a.by_per = inverse(a.per);
-  a.wg_tokens = std::max(1u, 256u / a.per);
+  // more than one where so many tokens need a launch of 2^32 lanes otherwise; a workgroup's units are divided by
+  // `per` in 32 bits
+  const unsigned most = (1u << 24) - 1;
+  a.wg_tokens = std::max({1u, 256u / a.per, (unsigned)(((unsigned long long)a.tokens + most - 1) / most)});
+  return (unsigned long long)a.wg_tokens * a.per * a.per < 1ULL << 32;
+}
+template <class T>
+hipError_t rotary(const rot::Args& a, bool interleaved, bool wide, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
   const dim3 grid((a.tokens + a.wg_tokens - 1) / a.wg_tokens), block(256);
   if (wide) {
     if (interleaved) hipLaunchKernelGGL((rot::rotary_kernel<T, V / 2, true>), grid, block, 0, st, a);
@@ -236,6 +242,7 @@ int sffft_rotary_apply(const sffft_rotary* p, const void* q, const void* k, cons
   for (int i = 0; i < 3; i++)
     wide = wide && p->q[i] * elem % 16 == 0 && p->qo[i] * elem % 16 == 0 &&
            (!k || (p->k[i] * elem % 16 == 0 && p->ko[i] * elem % 16 == 0));
+  if (!rotary_grid(a, elem, p->interleaved, wide)) return SFFFT_EINVAL;
   const auto run = p->io ? rotary<uint16_t> : rotary<float>;
   return ops::hip_status(run(a, p->interleaved, wide, (hipStream_t)stream), "rotary launch");
 }
@@ -279,7 +286,7 @@ int sffft_blocknorm_fwd(const sffft_blocknorm* p, const void* x, const void* y, 
   const RowShape s = row_shape(p, access_of(p, {{x, p->x}, {y, p->y}, {r, p->C}, {h, p->C}}, {gate, p->gate},
                                             {w_pre, w_post, scale}));
   const Parts q = parts_of(p, s, gate && p->gate_rows > 1, FILL_FWD);
-  if (q.nparts > INT_MAX) return SFFFT_EINVAL;
+  if (q.nparts > INT_MAX || !ops::launchable(q.nparts, 64 * s.waves)) return SFFFT_EINVAL;
   bn::Args a = {};
   a.x = x, a.y = y, a.gate = gate, a.sx = p->x, a.sy = p->y, a.sg = p->gate;
   a.wq = w_pre, a.wp = w_post, a.sc = scale, a.r = r, a.h = h;
@@ -326,7 +333,7 @@ int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, 
   const RowShape s = row_shape(p, access_of(p, {{x, p->x}, {y, p->y}, {gr, p->gr}, {gh, p->gh}, {dx, p->C}, {dy, p->C}, gates_out},
                                             gates_in, {w_pre, w_post, scale}));
   const Parts q = parts_of(p, s, shared, FILL_BWD);
-  if (q.nparts > INT_MAX) return SFFFT_EINVAL;
+  if (q.nparts > INT_MAX || !ops::launchable(q.nparts, 64 * s.waves)) return SFFFT_EINVAL;
   bn::Args a = {};
   a.x = x, a.y = y, a.gate = gate, a.gr = gr, a.gh = gh;
   a.sx = p->x, a.sy = p->y, a.sg = p->gate, a.sgr = p->gr, a.sgh = p->gh;
@@ -338,10 +345,11 @@ int sffft_blocknorm_bwd(const sffft_blocknorm* p, const void* x, const void* y, 
   const auto run = p->io ? norm<uint16_t> : norm<float>;
   hipError_t err = run(a, s, y != nullptr, true, dim3((unsigned)q.nparts), st);
   if (err == hipSuccess) {
-    const bn::SumArgs u = {a.parts, w_post, scale, dw_pre, dw_post, dscale, shared ? dgate : nullptr, p->C, p->io,
-                           y != nullptr, q.nparts, q.per_block};
     const long long sums = (y ? 2 : 1) + (shared ? q.blocks : 0);
-    hipLaunchKernelGGL(bn::sum_kernel, dim3((unsigned)((p->C + 31) / 32 * sums)), dim3(1024), 0, st, u);
+    const bn::SumArgs u = {a.parts, w_post, scale, dw_pre, dw_post, dscale, shared ? dgate : nullptr, p->C, p->io,
+                           y != nullptr, q.nparts, q.per_block, sums};
+    hipLaunchKernelGGL(bn::sum_kernel, dim3((unsigned)((p->C + 31) / 32), (unsigned)std::min<long long>(sums, 32768)), dim3(1024),
+                       0, st, u);
     err = hipGetLastError();
   }
   return ops::hip_status(err, "block norm gradient launch");

@@ -18,6 +18,9 @@ inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 inline bool aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 inline bool valid_io(int io) { return io == SFFFT_IO_F32 || io == SFFFT_IO_BF16; }
 
+// HIP takes no launch of 2^32 threads or more along a dimension.
+inline bool launchable(long long workgroups, int threads) { return workgroups < ((1LL << 32) + threads - 1) / threads; }
+
 // Bytes from the start of a strided [B][T][H][D] array to its end; 0 if an index may leave 62 bits or
 // a stride is negative.
 inline size_t extent(const long long s[3], int B, int T, int H, int D, int elem) {

@@ -41,7 +41,7 @@ using torch::autograd::variable_list;
 void* stream_of() { return c10::hip::getCurrentHIPStream().stream(); }
 
 void check(int rc, const char* what) {
-  TORCH_CHECK(rc == SFFFT_OK, what, " failed: error ", rc, rc == SFFFT_EHIP ? sffft_ops_last_error() : "");
+  TORCH_CHECK(rc == SFFFT_OK, what, " failed: ", sffft_strerror(rc), " (", rc, ") ", rc == SFFFT_EHIP ? sffft_ops_last_error() : "");
 }
 
 const void* ptr(const Tensor& t) { return t.defined() && t.numel() ? t.const_data_ptr() : nullptr; }
