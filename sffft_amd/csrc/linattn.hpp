@@ -585,7 +585,17 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
                                     [&](int n) -> auto& { return S[a + n / VW][n % VW]; });
       }
     }
-    if constexpr (OUT) stage_out();
+    if constexpr (OUT) {
+      // Tokens that do not count give 0, whatever the state holds: their rows of a are 0, but 0 times an infinity is not.
+      if (have < C) {
+#pragma unroll
+        for (int t = 0; t < MT; t++)
+#pragma unroll
+          for (int v = 0; v < VW; v++)
+            if (16 * t + i16 >= have) o[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      stage_out();
+    }
   }
   if constexpr (OUT) {
     if constexpr (VIA) ops::barrier();
