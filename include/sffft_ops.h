@@ -33,9 +33,9 @@ extern "C" {
  * S_{-1} is the initial state (zero if NULL); the final state is S_{n-1} (the initial one if n = 0).
  * States are [B][H][Dk][Dv] fp32. Tokens from n on are never read, whatever they hold. log_decay
  * <= 0 is meant (-inf: nothing is remembered); a positive one grows until it overflows. lengths
- * outside 0..T are taken as the nearest of these. Tokens are worked on in chunks of 64 (fp32: 32): an
- * infinity or NaN at one that counts may make NaN of the outputs of its whole chunk, and does of the later
- * ones; an infinity in fp32 counts as NaN. */
+ * outside 0..T are taken as the nearest of these. An infinity or NaN at a token that counts reaches the
+ * outputs that the definition lets it reach, no earlier tokens and no other channels; in later ones an
+ * infinity may count as NaN. */
 typedef struct sffft_linattn {
   int io;                 /* SFFFT_IO_F32 or SFFFT_IO_BF16: q, k, v, o and their gradients */
   int B, T, H, Hk;        /* H a multiple of Hk, at most 2^23 - 64 channels in all its heads */

@@ -37,6 +37,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16;
+typedef u16 u16x2 __attribute__((ext_vector_type(2)));
 
 // One operand: element strides of (batch, token, head); head h of the march reads head h / div.
 struct Operand {
@@ -233,6 +234,19 @@ struct Stage {
     for (int i = 0; i < N; i++)
       v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, row + i * ROWS < n ? at : OUTSIDE, i * ROWS * (int)st * (int)sizeof(T), 0);
   }
+  // whether no value is an infinity or NaN
+  __device__ __forceinline__ bool finite() const {
+    u16x2 top = {0, 0};
+    uint32_t top32 = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if constexpr (sizeof(T) == 2) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[i][k] & 0x7fff7fff));
+        else top32 = max(top32, (uint32_t)v[i][k] & 0x7fffffffu);
+      }
+    return sizeof(T) == 2 ? top.x < 0x7f80 && top.y < 0x7f80 : top32 < 0x7f800000u;
+  }
   // (tiles of 96 channels are fetched by the lanes of 128)
   template <int NS, int L>
   __device__ __forceinline__ void store(Tile<NS, C, L>& t) const {
@@ -274,10 +288,18 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   constexpr int LK = KT == 96 ? 128 : KT;  // lanes that fetch K channels take these
   // outputs leave through a's tile (below)
   constexpr bool VIA = OUT && NS == 1 && E == 2 && LK == VT;
-  __shared__ __attribute__((aligned(16))) Tile<NS, OUT ? C : 1, (VIA ? VT : KT) + 16> ta;
-  __shared__ __attribute__((aligned(16))) Tile<NS, C, KT + 16> tb;
-  __shared__ __attribute__((aligned(16))) Tile<NS, C, VT + 16> tc;
-  __shared__ __attribute__((aligned(16))) Tile<PX, OUT ? C : 1, C + 8, false> tp;  // PX: planes of P and X
+  struct Tiles {
+    Tile<NS, OUT ? C : 1, (VIA ? VT : KT) + 16> a;
+    Tile<NS, C, KT + 16> b;
+    Tile<NS, C, VT + 16> c;
+    Tile<PX, OUT ? C : 1, C + 8, false> p;  // PX: planes of P and X
+  };
+  __shared__ __attribute__((aligned(16))) Tiles tiles;
+  auto& ta = tiles.a;
+  auto& tb = tiles.b;
+  auto& tc = tiles.c;
+  auto& tp = tiles.p;
+  __shared__ int odd[2];  // whether this chunk, or the next, has infinities or NaN
   __shared__ __attribute__((aligned(16))) float fi[C], wj[C];  // decays: of the entering state at row i, of token j in the update
 
   // Workgroups go to the 8 XCDs in turn; the marches and V tiles of one head and segment, which read the same
@@ -305,9 +327,8 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   const bool back = OUT ? rev : !rev;
   const int dir = back ? -C : C;
   int t0 = back ? first + (chunks - 1) * C : first;
-  const T* pa = static_cast<const T*>(m.a.p) + b * m.a.sb + (h / m.a.div) * m.a.sh + t0 * m.a.st;
-  const T* pb = static_cast<const T*>(m.b.p) + b * m.b.sb + (h / m.b.div) * m.b.sh + t0 * m.b.st;
-  const T* pc = static_cast<const T*>(m.c.p) + b * m.c.sb + (h / m.c.div) * m.c.sh + t0 * m.c.st + v0;
+  auto token = [&](const Operand& x, int t) { return static_cast<const T*>(x.p) + b * x.sb + (h / x.div) * x.sh + t * x.st; };
+  const T *pa = token(m.a, t0), *pb = token(m.b, t0), *pc = token(m.c, t0) + v0;
   const int orow = L.s.H * m.V;
   TO* po = OUT ? static_cast<TO*>(m.out) + (((long long)b * L.s.T + t0) * L.s.H + h) * m.V : nullptr;
 
@@ -450,6 +471,55 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
     }
   };
 
+  // A chunk token by token, straight from memory: where a product is infinite or NaN the tiles of P that are 0 would
+  // carry it to tokens that must not see it. `from`: the chunk's first token, of which `count` count; rows: those of the
+  // output. The state goes through LDS, where the tiles are dead, so that no register is held for this.
+  auto by_token = [&](int from, int count, int rows) {
+    static_assert(!OUT || sizeof(tiles) >= KT * VT * sizeof(float), "");
+    float* X = reinterpret_cast<float*>(&tiles) + (w * KT + 4 * g) * 16 * VW + i16;
+#pragma unroll
+    for (int a = 0; a < KA; a++)
+#pragma unroll
+      for (int v = 0; v < VW; v++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) X[(16 * a + e) * 16 * VW + 16 * v] = S[a][v][e];
+    const float decay = power(1), before = rev ? 1.f : decay, after = rev ? decay : 1.f;
+    const T *ra = token(m.a, from) + 4 * g, *rb = token(m.b, from) + 4 * g, *rc = token(m.c, from) + sv0;
+#pragma unroll 1
+    for (int s = 0; s < rows; s++) {
+      const int i = rev && s < count ? count - 1 - s : s;
+      float sum[VW] = {}, c[VW];
+#pragma unroll
+      for (int v = 0; v < VW; v++) c[v] = s < count && sv0 + 16 * v < m.V ? m.w * ops::to_f32(rc[i * m.c.st + 16 * v]) : 0.f;
+#pragma unroll 1
+      for (int k = s < count ? 4 * g : m.K; k < m.K; k += 16)
+#pragma unroll 1
+        for (int e = 0; e < 4; e++) {
+          const float ak = ops::to_f32(ra[i * m.a.st + k - 4 * g + e]), bk = ops::to_f32(rb[i * m.b.st + k - 4 * g + e]);
+#pragma unroll
+          for (int v = 0; v < VW; v++) {
+            float& x = X[(k - 4 * g + e) * 16 * VW + 16 * v];
+            const float y = x * before + bk * c[v];
+            sum[v] += ak * y;
+            x = y * after;
+          }
+        }
+#pragma unroll
+      for (int v = 0; v < VW; v++) {
+        sum[v] += __shfl_xor(sum[v], 16);
+        sum[v] += __shfl_xor(sum[v], 32);
+        if (g == 0 && sv0 + 16 * v < m.V) ops::put(po + (long long)i * orow + sv0 + 16 * v, m.x * sum[v]);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < KA; a++)
+#pragma unroll
+      for (int v = 0; v < VW; v++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) S[a][v][e] = X[(16 * a + e) * 16 * VW + 16 * v];
+  };
+
+  if (threadIdx.x == 0) odd[0] = 0;
   float gn = 1.f;
   int have = OUT ? -1 : 0;  // tokens of the chunk that the decays are for; of the chunks before
   for (int c = 0; c < chunks; c++) {
@@ -462,6 +532,8 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
     }
     gb.store(tb);
     gc.store(tc);
+    if constexpr (OUT)
+      if (!gc.finite()) odd[c & 1] = 1;
     // The decays depend on the tokens in a chunk; in the sums also on those between the chunk and where the sum is
     // taken.
     if (!OUT || n != have) {
@@ -479,6 +551,8 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
     ops::barrier();
 
     if constexpr (OUT) {
+      if (threadIdx.x == 0) odd[~c & 1] = 0;
+      bool finite = true;  // so are a and b if their products with tokens of their own are
       // P^T tiles: rows j, columns i
 #pragma unroll
       for (int t = 0; t < NP; t++) {
@@ -491,6 +565,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
         // stored in the order of the transposing reads' rows: 16 * (j / 16 % 2) + 4 g + e at 8 g + 4 (j / 16 % 2) + e
         u16* q = &tp.v[0][16 * pi[t] + i16][32 * (pj[t] >> 1) + 8 * g + 4 * (pj[t] & 1)];
         const float x0 = d[0] * pd[t][0], x1 = d[1] * pd[t][1], x2 = d[2] * pd[t][2], x3 = d[3] * pd[t][3];
+        finite = finite && __builtin_isfinite(x0) && __builtin_isfinite(x1) && __builtin_isfinite(x2) && __builtin_isfinite(x3);
         if constexpr (PX == 2) {
           uint2 hh, mm;
           split2(x0, x1, hh.x, mm.x);
@@ -506,6 +581,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
           *reinterpret_cast<uint2*>(q + 2 * C * (C + 8)) = ll;
         }
       }
+      if (!finite) odd[c & 1] = 1;
       // a X, transposed: rows vv, columns i
 #pragma unroll
       for (int t = 0; t < MT; t++)
@@ -534,6 +610,11 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
         for (int v = 0; v < VW; v++) o[t][v] *= f;
       }
       ops::barrier();
+      if (__builtin_amdgcn_readfirstlane(odd[c & 1])) {
+        by_token(t0 - dir, have, min(left, C));
+        left = 0;  // the outputs have left
+        continue;
+      }
     }
 
     if constexpr (OUT)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import mixer_oracle as mo
 from sffft_amd import torch_ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,25 @@ def test_tokens_that_do_not_count_give_zero_whatever_the_states_hold(dev, T, len
     for b, m in enumerate(lengths):
         if m == 0:
             assert torch.equal(got["state"][b], s0[b]) and torch.equal(got["dstate"][b].nan_to_num(1), gs[b].nan_to_num(1))
+
+
+@DTYPES
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+@pytest.mark.parametrize("where", ["q", "k", "v", "go"])
+@pytest.mark.parametrize("B,T,H,Hk,Dk,Dv,token,lengths", [(1, 1, 1, 1, 8, 8, 0, None), (2, 150, 2, 1, 64, 64, 70, [150, 100]),
+                                                         (1, 90, 2, 2, 24, 128, 33, None), (1, 640, 2, 2, 128, 128, 300, None),
+                                                         (1, 70, 2, 1, 96, 72, 64, None), (1, 130, 1, 1, 128, 40, 127, [129])])
+def test_one_value_reaches_what_the_definition_lets_it_reach(dev, B, T, H, Hk, Dk, Dv, token, lengths, where, value, dtype):
+    """The finite places are those of the 64-bit recurrence and its gradients, with values as near as ever: a value
+    that is not finite stays away from the tokens before its own (after it, in the gradients of keys and values), and
+    from channels that it has no part in."""
+    q, k, v, ld, s0, go, gs = inputs(dev, B, T, H, Hk, Dk, Dv, dtype, seed=token)
+    x = {"q": q, "k": k, "v": v, "go": go}[where]
+    x[0, token, 0, 5] = value
+    want = mo.attention_grads(q, k, v, ld, 0.2, go, gs, s0, lengths)
+    got = run(q, k, v, ld, s0, go, gs, None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=dev))
+    for (name, a), w in zip(got.items(), want):
+        a = a.double().cpu()
+        assert torch.equal(torch.isfinite(a), torch.isfinite(w)), name
+        bound = 3 * 2.0 ** -9 if dtype == torch.bfloat16 and name not in ("state", "dstate") else 1e-5
+        assert mo.rel_l2(torch.where(torch.isfinite(w), a, 0.0), torch.where(torch.isfinite(w), w, 0.0)) < bound, name
