@@ -32,7 +32,7 @@ extern "C" {
  *   S_t = g S_{t-1} + k_t v_t^T (t < n),   o_t = scale S_t^T q_t (t < n; 0 from n on)
  * S_{-1} is the initial state (zero if NULL); the final state is S_{n-1} (the initial one if n = 0).
  * States are [B][H][Dk][Dv] fp32. Tokens from n on are never read, whatever they hold. log_decay
- * <= 0 is meant (-inf: nothing is remembered); a positive one grows until it overflows. lengths
+ * <= 0 is meant (-inf: nothing is remembered); a positive one grows until it overflows, NaN makes NaN. lengths
  * outside 0..T are taken as the nearest of these. An infinity or NaN at a token that counts reaches the
  * outputs that the definition lets it reach, no earlier tokens and no other channels; in later ones an
  * infinity may count as NaN. */

@@ -80,8 +80,15 @@ struct Launch {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// log2 of the decay; -inf becomes a finite value whose powers are 0, so that the zeroth is 1
-__device__ __forceinline__ float decay_log2(const float* log_decay, int h) { return fmaxf(log_decay[h] * LOG2E, -1e4f); }
+// log2 of the decay; -inf becomes a finite value whose powers are 0. NaN stays (fmaxf would drop it).
+__device__ __forceinline__ float decay_log2(const float* log_decay, int h) {
+  const float x = log_decay[h] * LOG2E;
+  return x < -1e4f ? -1e4f : x;
+}
+// the decay over n tokens: 1 over none, whatever it is; 0 for negative n
+__device__ __forceinline__ float decay_power(float l2, int n) {
+  return n < 0 ? 0.f : __builtin_amdgcn_exp2f(n == 0 ? 0.f : l2 * (float)n);
+}
 __device__ __forceinline__ int valid_tokens(const Shape& s, int b) {
   return s.lengths ? min(max(s.lengths[b], 0), s.T) : s.T;
 }
@@ -319,7 +326,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   const int first = z * L.seg, last = first + min(L.seg, L.s.T - first), chunks = (last - first + C - 1) / C;
   const int end = min(valid_tokens(L.s, b), last);  // of the tokens that count
   const float l2 = decay_log2(L.s.log_decay, h);
-  auto power = [&](int n) { return n < 0 ? 0.f : __builtin_amdgcn_exp2f(l2 * (float)n); };
+  auto power = [&](int n) { return decay_power(l2, n); };
   auto count = [&](int t0) { return __builtin_amdgcn_readfirstlane(min(max(end - t0, 0), C)); };
 
   // The first chunk: the last one of the segment if reversed. The sums go the other way, so that what they read last
@@ -719,7 +726,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
     for (int i = 0; i < AHEAD; i++)
       if (z0 + i < L.nseg) {
         const int z = c.rev ? L.nseg - 1 - z0 - i : z0 + i;
-        const float d = __builtin_amdgcn_exp2f(l2 * (float)min(max(valid - z * L.seg, 0), L.seg));
+        const float d = decay_power(l2, min(max(valid - z * L.seg, 0), L.seg));
         ops::store(p + (long long)z * c.n, x);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = x[k] * d + u[i][k];
@@ -776,7 +783,7 @@ __global__ __launch_bounds__(256) void step_kernel(Operand q, Operand k, Operand
   const bool live = row >= 0 && row < slots, in = col < Dv;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   if (live && in) {
-    const float g = exp2f(fmaxf(log_decay[h] * LOG2E, -1e4f));
+    const float g = exp2f(decay_log2(log_decay, h));
     const T* qp = static_cast<const T*>(q.p) + b * q.sb + (h / q.div) * q.sh;
     const T* kp = static_cast<const T*>(k.p) + b * k.sb + (h / k.div) * k.sh;
     const T* vp = static_cast<const T*>(v.p) + b * v.sb + (h / v.div) * v.sh;

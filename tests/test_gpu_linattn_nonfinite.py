@@ -65,3 +65,42 @@ def test_one_value_reaches_what_the_definition_lets_it_reach(dev, B, T, H, Hk, D
         assert torch.equal(torch.isfinite(a), torch.isfinite(w)), name
         bound = 3 * 2.0 ** -9 if dtype == torch.bfloat16 and name not in ("state", "dstate") else 1e-5
         assert mo.rel_l2(torch.where(torch.isfinite(w), a, 0.0), torch.where(torch.isfinite(w), w, 0.0)) < bound, name
+
+
+@DTYPES
+@pytest.mark.parametrize("B,T,lengths", [(2, 1, [1, 0]), (2, 90, [90, 33]), (2, 900, [900, 0]), (1, 4000, [3999])])
+def test_a_decay_of_nan_is_not_hidden(dev, B, T, lengths, dtype):
+    """It makes NaN of what its head's decay reaches, and of nothing else: the other heads keep their bits."""
+    H, D = 4, 64
+    q, k, v, ld, s0, go, gs = inputs(dev, B, T, H, H, D, D, dtype, seed=T)
+    n = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    want = run(q, k, v, ld, s0, go, gs, n)
+    bad = ld.clone()
+    bad[2] = NAN
+    got = run(q, k, v, bad, s0, go, gs, n)
+    others = [0, 1, 3]
+    for name in got:
+        h = 1 if name in ("state", "dstate") else 2
+        assert torch.equal(got[name].index_select(h, torch.tensor(others, device=dev)),
+                           want[name].index_select(h, torch.tensor(others, device=dev))), name
+    for b, m in enumerate(lengths):
+        assert bool(torch.isnan(got["o"][b, :m, 2]).all()) and bool(torch.isnan(got["dq"][b, :m, 2]).all())
+        assert not bool(got["o"][b, m:].any())
+        if m:
+            assert bool(torch.isnan(got["state"][b, 2]).all()) and bool(torch.isnan(got["dstate"][b, 2]).all())
+            # the last token's key and value do not pass a decay on their way to the final state
+            assert bool(torch.isnan(got["dk"][b, :m - 1, 2]).all()) and bool(torch.isfinite(got["dk"][b, m - 1, 2]).all())
+            assert bool(torch.isnan(got["dv"][b, :m - 1, 2]).all()) and bool(torch.isfinite(got["dv"][b, m - 1, 2]).all())
+        else:
+            assert torch.equal(got["state"][b], s0[b]) and torch.equal(got["dstate"][b], gs[b])
+
+
+@DTYPES
+def test_a_decay_of_nan_is_not_hidden_from_single_tokens(dev, dtype):
+    q, k, v, ld, s0, _, _ = inputs(dev, 3, 1, 4, 2, 64, 32, dtype)
+    want, bad = s0.clone(), s0.clone()
+    o = torch.ops.sffft.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, want, 0.2)
+    ld[1] = NAN
+    p = torch.ops.sffft.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, bad, 0.2)
+    for x, y in ((p, o), (bad, want)):
+        assert bool(torch.isnan(x[:, 1]).all()) and torch.equal(x[:, [0, 2, 3]], y[:, [0, 2, 3]])
