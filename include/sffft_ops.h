@@ -77,7 +77,8 @@ int sffft_linattn_step(const sffft_linattn* p, const void* q, const void* k, con
  * inverse = 1 by the negative angle (the gradient). Token t of sequence b has position
  * pos[b][t] (pos_bits 32 or 64), t if pos is NULL; a position outside the table gives NaN in the
  * rotated channels and reads nothing. (H + Hk) * D / 2 is at most 65535. qo may be q and ko k, with
- * equal strides; else they overlap neither. */
+ * equal strides; else they overlap neither. No two elements of the outputs, nor one of an output in place
+ * and one of the other input, are the same; q and k may be parts of one array. */
 typedef struct sffft_rotary {
   int io;
   int B, T, H, Hk, D;

@@ -221,7 +221,13 @@ int sffft_rotary_apply(const sffft_rotary* p, const void* q, const void* k, cons
   // in place (q itself, with its strides) or apart
   const bool sq = q == qo && std::equal(p->q, p->q + 3, p->qo), sk = k == ko && std::equal(p->k, p->k + 3, p->ko);
   const size_t nt = (size_t)p->positions * p->R * 4, np = pos ? (size_t)p->B * p->T * (p->pos_bits / 8) : 0;
-  // (in place, q and k may be views of one array whose extents interleave)
+  // (q and k may be views of one array whose extents interleave; what is written in place is no element of another)
+  const auto apart_from = [&](const void* a, const long long* sa, int ha, const void* b, const long long* sb, int hb) {
+    return ops::distinct(a, sa, ha, b, sb, hb, p->B, p->T, p->D, elem);
+  };
+  if (!apart_from(qo, p->qo, p->H, ko, p->ko, p->Hk) || (sq && !apart_from(q, p->q, p->H, k, p->k, p->Hk)) ||
+      (sk && k && !apart_from(k, p->k, p->Hk, q, p->q, p->H)))
+    return SFFFT_EINVAL;
   if ((!sq && (ops::overlap(qo, mq, q, nq) || ops::overlap(qo, mq, k, k ? nk : 0))) ||
       (!sk && (ops::overlap(ko, mk, k, nk) || ops::overlap(ko, k ? mk : 0, q, nq))) || qo == ko ||
       ops::overlap(qo, mq, table, nt) ||

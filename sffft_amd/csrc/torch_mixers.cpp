@@ -247,9 +247,11 @@ void rotary_run(const Tensor& q, const Tensor& k, const Tensor& table_in, const 
   p.B = (int)B, p.T = (int)T, p.H = (int)a.size(2), p.Hk = (int)c.size(2), p.D = (int)a.size(3);
   p.R = (int)table.size(1), p.interleaved = interleaved, p.inverse = inverse, p.positions = (int)table.size(0);
   for (int i = 0; i < 3; i++) p.q[i] = a.stride(i), p.k[i] = c.stride(i), p.qo[i] = ao.stride(i), p.ko[i] = co.stride(i);
-  check(sffft_rotary_apply(&p, ptr(a), ptr(c), table.const_data_ptr<float>(), ptr(pos), ao.data_ptr(),
-                           p.Hk ? co.data_ptr() : nullptr, stream_of()),
-        ROT);
+  const int rc = sffft_rotary_apply(&p, ptr(a), ptr(c), table.const_data_ptr<float>(), ptr(pos), ao.data_ptr(),
+                                    p.Hk ? co.data_ptr() : nullptr, stream_of());
+  TORCH_CHECK(rc != SFFFT_EINVAL || !ao.is_same(a), ROT, "_: q and k may overlap neither themselves nor each other, nor the table "
+              "or positions; got strides ", q.strides(), " and ", k.strides());
+  check(rc, ROT);
 }
 
 Tensor channels_last(const Tensor& t) {
@@ -269,12 +271,9 @@ std::tuple<Tensor, Tensor> rotary_gpu(const Tensor& q, const Tensor& k, const Te
 void rotary_inplace_gpu(const Tensor& q, const Tensor& k, const Tensor& table, const OptTensor& positions,
                         bool interleaved) {
   const c10::DeviceGuard guard(q.device());
-  for (const Tensor* t : {&q, &k}) {
+  for (const Tensor* t : {&q, &k})
     TORCH_CHECK(t->dim() == 4 && (t->numel() == 0 || t->stride(3) == 1), ROT,
                 "_: q and k must be [B, T, H, D] with contiguous channels, got ", t->sizes(), " strides ", t->strides());
-    for (int d = 0; d < 3; d++)
-      TORCH_CHECK(t->size(d) <= 1 || t->stride(d) >= t->size(3), ROT, "_: q and k may not overlap themselves");
-  }
   rotary_run(q, k, table, positions, interleaved, false, q, k);
 }
 
