@@ -236,17 +236,17 @@ int sffft_linattn_fwd(const sffft_linattn* p, const void* q, const void* k, cons
       !ops::aligned(lengths, 4))
     return SFFFT_EINVAL;
   const size_t no = (size_t)p->B * p->T * p->H * p->Dv * (p->io ? 2 : 4), ns = (size_t)p->B * p->H * p->Dk * p->Dv * 4;
-  const void* in[] = {q, k, v, initial_state};
-  const size_t len[] = {nq, nk, nv, ns};
-  for (int i = 0; i < 4; i++)
-    if (ops::overlap(o, no, in[i], len[i]) || ((i < 3 || in[i] != final_state) && ops::overlap(final_state, ns, in[i], len[i])))
+  const void* in[] = {q, k, v, initial_state, log_decay, lengths};
+  const size_t len[] = {nq, nk, nv, ns, (size_t)p->H * 4, (size_t)p->B * 4};
+  for (int i = 0; i < 6; i++)
+    if (ops::overlap(o, no, in[i], len[i]) || ((i != 3 || in[i] != final_state) && ops::overlap(final_state, ns, in[i], len[i])))
       return SFFFT_EINVAL;
   if (ops::overlap(o, no, final_state, ns)) return SFFFT_EINVAL;
   const size_t need = sffft_linattn_work_bytes(p, 0);
   if (need && (!work || work_bytes < need || !ops::aligned(work, 16) || ops::overlap(work, need, o, no) ||
                ops::overlap(work, need, final_state, ns)))
     return SFFFT_EINVAL;
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < 6; i++)
     if (need && ops::overlap(work, need, in[i], len[i])) return SFFFT_EINVAL;
   const Shape s = {p->B, p->T, p->H, log_decay, lengths};
   const auto run = p->io ? forward<uint16_t> : forward<float>;
@@ -268,12 +268,12 @@ int sffft_linattn_bwd(const sffft_linattn* p, const void* q, const void* k, cons
   const size_t elem = p->io ? 2 : 4, rows = (size_t)p->B * p->T, ns = (size_t)p->B * p->H * p->Dk * p->Dv * 4;
   const size_t need = sffft_linattn_work_bytes(p, 1);
   if (need && (!work || work_bytes < need || !ops::aligned(work, 16))) return SFFFT_EINVAL;
-  const void* in[] = {q, k, v, go, initial_state, d_final_state};
-  const size_t len[] = {nq, nk, nv, no, ns, ns};
+  const void* in[] = {q, k, v, go, initial_state, d_final_state, log_decay, lengths};
+  const size_t len[] = {nq, nk, nv, no, ns, ns, (size_t)p->H * 4, (size_t)p->B * 4};
   const void* out[] = {dq, dk, dv, d_initial_state, need ? work : nullptr};
   const size_t size[] = {rows * p->H * p->Dk * elem, rows * p->Hk * p->Dk * elem, rows * p->Hk * p->Dv * elem, ns, need};
   for (int i = 0; i < 5; i++) {
-    for (int j = 0; j < 6; j++)
+    for (int j = 0; j < 8; j++)
       if (ops::overlap(out[i], size[i], in[j], len[j])) return SFFFT_EINVAL;
     for (int j = 0; j < i; j++)
       if (ops::overlap(out[i], size[i], out[j], size[j])) return SFFFT_EINVAL;
@@ -294,9 +294,9 @@ int sffft_linattn_step(const sffft_linattn* p, const void* q, const void* k, con
       !ops::aligned(log_decay, 4) || !ops::aligned(slot, 4))
     return SFFFT_EINVAL;
   const size_t no = (size_t)p->B * p->H * p->Dv * (p->io ? 2 : 4), ns = (size_t)slots * p->H * p->Dk * p->Dv * 4;
-  const void* in[] = {q, k, v};
-  const size_t len[] = {nq, nk, nv};
-  for (int i = 0; i < 3; i++)
+  const void* in[] = {q, k, v, log_decay, slot};
+  const size_t len[] = {nq, nk, nv, (size_t)p->H * 4, (size_t)p->B * 4};
+  for (int i = 0; i < 5; i++)
     if (ops::overlap(o, no, in[i], len[i]) || ops::overlap(state, ns, in[i], len[i])) return SFFFT_EINVAL;
   if (ops::overlap(o, no, state, ns)) return SFFFT_EINVAL;
   const int G = p->H / p->Hk;
