@@ -89,6 +89,28 @@ __device__ __forceinline__ float decay_log2(const float* log_decay, int h) {
 __device__ __forceinline__ float decay_power(float l2, int n) {
   return n < 0 ? 0.f : __builtin_amdgcn_exp2f(n == 0 ? 0.f : l2 * (float)n);
 }
+// The decay over n tokens for states that pass it many times over. Rounded to fp32 it would be off by the same part of
+// itself each time, 1e-4 after 4096 chunks of a slow head; next() makes up in each factor for what the ones before it
+// left out. (A head that forgets half of its state or more in n tokens keeps no such error.)
+struct Decay {
+  float hi, lo, inv;  // the decay is hi + lo
+  __device__ __forceinline__ Decay(const float* log_decay, int h, int n) {
+    float e = n == 0 ? 0.f : expm1f(log_decay[h] * (float)n);
+    e = e > 3e38f ? 3e38f : e;
+    const bool slow = e > -0.5f;
+    const float g = slow ? 1.f + e : decay_power(decay_log2(log_decay, h), n);
+    hi = uniform(g), lo = uniform(slow && e <= 1.f ? e - (g - 1.f) : 0.f), inv = uniform(slow ? 1.f / g : 0.f);
+  }
+  static __device__ __forceinline__ float uniform(float x) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+  }
+  // the next factor; `behind`: by what part of it the product so far is too small
+  __device__ __forceinline__ float next(float& behind) const {
+    const float t = lo + hi * behind, g = hi + t;
+    behind = (t - (g - hi)) * inv;
+    return g;
+  }
+};
 __device__ __forceinline__ int valid_tokens(const Shape& s, int b) {
   return s.lengths ? min(max(s.lengths[b], 0), s.T) : s.T;
 }
@@ -527,7 +549,8 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   };
 
   if (threadIdx.x == 0) odd[0] = 0;
-  float gn = 1.f;
+  Decay gn(L.s.log_decay, h, 0);
+  float behind = 0.f;
   int have = OUT ? -1 : 0;  // tokens of the chunk that the decays are for; of the chunks before
   for (int c = 0; c < chunks; c++) {
     ops::barrier();
@@ -549,7 +572,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
         if constexpr (OUT) fi[i] = m.x * power(rev ? n - 1 - i : i + 1);
         wj[i] = m.w * power(i >= n ? -1 : behind + (rev ? i + 1 : n - 1 - i));
       }
-      if constexpr (OUT) have = n, gn = power(n);
+      if constexpr (OUT) have = n, gn = Decay(L.s.log_decay, h, n);
       else have += n;
     }
     t0 += dir;
@@ -624,11 +647,13 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
       }
     }
 
-    if constexpr (OUT)
+    if constexpr (OUT) {
+      const float f = gn.next(behind);
 #pragma unroll
       for (int a = 0; a < KA; a++)
 #pragma unroll
-        for (int v = 0; v < VW; v++) S[a][v] *= gn;
+        for (int v = 0; v < VW; v++) S[a][v] *= f;
+    }
 #pragma unroll
     for (int s = 0; s < JS; s++) {
       // c's channels as an operand, tokens along the sum; and decayed, to be added to the state
@@ -712,7 +737,9 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
   const int tiles = (c.n + 1023) / 1024, bh = blockIdx.x / tiles, e = ((blockIdx.x - bh * tiles) * 256 + threadIdx.x) * 4;
   if (e >= c.n) return;
   const int h = bh % L.s.H, b = bh / L.s.H, valid = valid_tokens(L.s, b);
-  const float l2 = decay_log2(L.s.log_decay, h);
+  // of a whole segment, and of the one that the sequence ends in
+  const Decay whole(L.s.log_decay, h, L.seg), part(L.s.log_decay, h, valid % L.seg);
+  float behind = 0.f;
   float x[4] = {0.f, 0.f, 0.f, 0.f};
   if (c.s0) ops::load(c.s0 + (long long)bh * c.n + e, x);
   float* p = c.sums + (long long)bh * L.nseg * c.n + e;
@@ -726,7 +753,8 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanLaunch L) {
     for (int i = 0; i < AHEAD; i++)
       if (z0 + i < L.nseg) {
         const int z = c.rev ? L.nseg - 1 - z0 - i : z0 + i;
-        const float d = decay_power(l2, min(max(valid - z * L.seg, 0), L.seg));
+        const int n = min(max(valid - z * L.seg, 0), L.seg);
+        const float d = n == L.seg ? whole.next(behind) : n ? part.hi : 1.f;
         ops::store(p + (long long)z * c.n, x);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = x[k] * d + u[i][k];
