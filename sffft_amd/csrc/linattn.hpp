@@ -811,7 +811,7 @@ __global__ __launch_bounds__(256) void step_kernel(Operand q, Operand k, Operand
   const bool live = row >= 0 && row < slots, in = col < Dv;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   if (live && in) {
-    const float g = exp2f(decay_log2(log_decay, h));
+    const Decay g(log_decay, h, 1);  // in two parts: calls that follow each other would add up the rounding of one
     const T* qp = static_cast<const T*>(q.p) + b * q.sb + (h / q.div) * q.sh;
     const T* kp = static_cast<const T*>(k.p) + b * k.sb + (h / k.div) * k.sh;
     const T* vp = static_cast<const T*>(v.p) + b * v.sb + (h / v.div) * v.sh;
@@ -828,7 +828,7 @@ __global__ __launch_bounds__(256) void step_kernel(Operand q, Operand k, Operand
         const float kv = ops::to_f32(kp[kk]), qv = ops::to_f32(qp[kk]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          x[i][e] = g * x[i][e] + kv * vv[e];
+          x[i][e] = __builtin_fmaf(g.hi, x[i][e], __builtin_fmaf(g.lo, x[i][e], kv * vv[e]));
           acc[e] += qv * x[i][e];
         }
         ops::store(sp + (long long)kk * Dv, x[i]);

@@ -71,3 +71,22 @@ def test_decays_of_every_speed(dev, dtype):
     want = torch.exp(ld.double() * T)[None, :, None, None] * s0.double()
     # products of decays in the exponent: 2^-24 of 0.3 * 224 = 67
     assert float(((s.double() - want).abs() / want.abs()).max()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_states_after_many_single_tokens(dev, dtype):
+    """The decay of a token, rounded, would be off by up to 2^-24 in one direction each time: 2.4e-4 after 4096. A token
+    rounds the state once or twice: 2^-25 sqrt(8192) = 3e-6 of a head's state, an eighth of it along the state, and
+    the decay 2^-23 of its argument, 0.2 in all; 1e-5 and 2e-6 are allowed."""
+    H, D, n = 64, 8, 4096
+    g = torch.Generator(device=dev).manual_seed(3)
+    ld = -torch.logspace(-6.2, -4.3, H, device=dev)
+    q, k, v = (torch.randn(n, 1, H, D, generator=g, device=dev).to(dtype) for _ in range(3))
+    s0 = torch.randn(1, H, D, D, generator=g, device=dev) * 1e5
+    s = s0.clone()
+    for t in range(n):
+        torch.ops.sffft.linear_attention_step(q[t], k[t], v[t], ld, s, 0.3)
+    _, last = oracle(*(x.transpose(0, 1) for x in (q, k, v)), ld, s0, 0.3)
+    d = (s.double() - last).flatten(2).norm(dim=2) / last.flatten(2).norm(dim=2)
+    along = (s.double() * last).flatten(2).sum(2) / (last * last).flatten(2).sum(2) - 1
+    assert float(d.max()) < 1e-5 and float(along.abs().max()) < 2e-6, (float(d.max()), float(along.abs().max()))
