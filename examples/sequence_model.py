@@ -108,6 +108,8 @@ class Model(torch.nn.Module):
 
     def run(self, tokens, mix):
         """mix(i, block, h) gives a block's output and gate."""
+        if tokens.shape[1] > self.length:
+            raise ValueError(f"at most {self.length} tokens, got {tokens.shape[1]}")
         x = F.embedding(tokens, self.embed.to(BF16))
         h = ops.pre_norm(x, self.pre[0])
         for i, block in enumerate(self.mixers):
@@ -137,6 +139,11 @@ class Model(torch.nn.Module):
     @torch.no_grad()
     def generate(self, tokens, lengths, n):
         """n more tokens, the likeliest each, of prompts tokens[b, :lengths[b]]; with the logits they were taken from."""
+        shortest, longest = int(lengths.min()), int(lengths.max())
+        if shortest < 1:
+            raise ValueError("an empty prompt has no last token to go on from")
+        if longest > tokens.shape[1] or longest + n - 1 > self.length:
+            raise ValueError(f"prompts of {longest} tokens in {tokens.shape[1]} and {n} more: the blocks keep {self.length}")
         logits, kept = self.prompt(tokens, lengths)
         last = logits[torch.arange(tokens.shape[0], device=tokens.device), lengths.long() - 1]
         out, seen = [], []
