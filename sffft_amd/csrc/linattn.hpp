@@ -502,50 +502,43 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
 
   // A chunk token by token, straight from memory: where a product is infinite or NaN the tiles of P that are 0 would
   // carry it to tokens that must not see it. `from`: the chunk's first token, of which `count` count; rows: those of the
-  // output. The state goes through LDS, where the tiles are dead, so that no register is held for this.
+  // output. The state goes through LDS, 16 columns of a wavefront at a time, where the tiles of a, b and c are dead
+  // (P's keep their zeros), so that no register is held for this.
   auto by_token = [&](int from, int count, int rows) {
-    static_assert(!OUT || sizeof(tiles) >= KT * VT * sizeof(float), "");
-    float* X = reinterpret_cast<float*>(&tiles) + (w * KT + 4 * g) * 16 * VW + i16;
-#pragma unroll
-    for (int a = 0; a < KA; a++)
-#pragma unroll
-      for (int v = 0; v < VW; v++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) X[(16 * a + e) * 16 * VW + 16 * v] = S[a][v][e];
+    static_assert(!OUT || sizeof(tiles) - sizeof(tp) >= KT * 64 * sizeof(float), "");
+    float* X = reinterpret_cast<float*>(&tiles) + (w * KT + 4 * g) * 16 + i16;
     const float decay = power(1), before = rev ? 1.f : decay, after = rev ? decay : 1.f;
-    const T *ra = token(m.a, from) + 4 * g, *rb = token(m.b, from) + 4 * g, *rc = token(m.c, from) + sv0;
-#pragma unroll 1
-    for (int s = 0; s < rows; s++) {
-      const int i = rev && s < count ? count - 1 - s : s;
-      float sum[VW] = {}, c[VW];
 #pragma unroll
-      for (int v = 0; v < VW; v++) c[v] = s < count && sv0 + 16 * v < m.V ? m.w * ops::to_f32(rc[i * m.c.st + 16 * v]) : 0.f;
-#pragma unroll 1
-      for (int k = s < count ? 4 * g : m.K; k < m.K; k += 16)
-#pragma unroll 1
-        for (int e = 0; e < 4; e++) {
-          const float ak = ops::to_f32(ra[i * m.a.st + k - 4 * g + e]), bk = ops::to_f32(rb[i * m.b.st + k - 4 * g + e]);
+    for (int v = 0; v < VW; v++) {
 #pragma unroll
-          for (int v = 0; v < VW; v++) {
-            float& x = X[(k - 4 * g + e) * 16 * VW + 16 * v];
-            const float y = x * before + bk * c[v];
-            sum[v] += ak * y;
+      for (int a = 0; a < KA; a++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) X[(16 * a + e) * 16] = S[a][v][e];
+      const int vv = sv0 + 16 * v;
+      const T *ra = token(m.a, from) + 4 * g, *rb = token(m.b, from) + 4 * g, *rc = token(m.c, from) + vv;
+#pragma unroll 1
+      for (int s = 0; s < rows; s++) {
+        const int i = rev && s < count ? count - 1 - s : s;
+        const float c = s < count && vv < m.V ? m.w * ops::to_f32(rc[i * m.c.st]) : 0.f;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int k = s < count ? 4 * g : m.K; k < m.K; k += 16)
+#pragma unroll 1
+          for (int e = 0; e < 4; e++) {
+            float& x = X[(k - 4 * g + e) * 16];
+            const float y = x * before + ops::to_f32(rb[i * m.b.st + k - 4 * g + e]) * c;
+            sum += ops::to_f32(ra[i * m.a.st + k - 4 * g + e]) * y;
             x = y * after;
           }
-        }
-#pragma unroll
-      for (int v = 0; v < VW; v++) {
-        sum[v] += __shfl_xor(sum[v], 16);
-        sum[v] += __shfl_xor(sum[v], 32);
-        if (g == 0 && sv0 + 16 * v < m.V) ops::put(po + (long long)i * orow + sv0 + 16 * v, m.x * sum[v]);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (g == 0 && vv < m.V) ops::put(po + (long long)i * orow + vv, m.x * sum);
       }
+#pragma unroll
+      for (int a = 0; a < KA; a++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) S[a][v][e] = X[(16 * a + e) * 16];
     }
-#pragma unroll
-    for (int a = 0; a < KA; a++)
-#pragma unroll
-      for (int v = 0; v < VW; v++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) S[a][v][e] = X[(16 * a + e) * 16 * VW + 16 * v];
   };
 
   if (threadIdx.x == 0) odd[0] = 0;

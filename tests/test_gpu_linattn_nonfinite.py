@@ -104,3 +104,34 @@ def test_a_decay_of_nan_is_not_hidden_from_single_tokens(dev, dtype):
     p = torch.ops.sffft.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, bad, 0.2)
     for x, y in ((p, o), (bad, want)):
         assert bool(torch.isnan(x[:, 1]).all()) and torch.equal(x[:, [0, 2, 3]], y[:, [0, 2, 3]])
+
+
+@DTYPES
+@pytest.mark.parametrize("B,T,H,Hk,Dk,Dv", [(60, 330, 12, 12, 128, 128), (60, 330, 12, 4, 128, 128), (60, 330, 12, 4, 96, 128), (100, 330, 12, 12, 64, 64),
+                                            (100, 330, 12, 6, 32, 64), (60, 200, 12, 12, 64, 128)])
+def test_chunks_after_one_that_is_not_finite(dev, B, T, H, Hk, Dk, Dv, dtype):
+    """In a march of several chunks the others come out as without it, wherever the value has no part."""
+    q, k, v, ld, s0, go, gs = inputs(dev, B, T, H, Hk, Dk, Dv, dtype, seed=7)
+    clean, t = run(q, k, v, ld, s0, go, gs), 70
+    channels = [c for c in range(Dv) if c != 5]
+
+    def near(a, b):  # two roundings to bf16 (2^-9 each, root mean square); fp32 in another order of the sums
+        a, b = a.double(), b.double()
+        return bool(torch.isfinite(a).all()) and float((a - b).norm() / b.norm()) < (2.0 ** -8 if dtype == torch.bfloat16 else 1e-5)
+
+    w = v.clone()
+    w[:, t, :, 5] = INF
+    got = run(q, k, w, ld, s0, go, gs)
+    assert near(got["o"][..., channels], clean["o"][..., channels]) and near(got["o"][:, :t], clean["o"][:, :t])
+    assert near(got["state"][..., channels], clean["state"][..., channels])
+    assert near(got["dq"][:, :t], clean["dq"][:, :t]) and near(got["dv"], clean["dv"]) and near(got["dstate"], clean["dstate"])
+    others = [i for i in range(T) if i != t]
+    assert near(got["dk"][:, others], clean["dk"][:, others])
+    assert not bool(torch.isfinite(got["o"][:, t:, :, 5]).any())
+    w = go.clone()
+    w[:, t, :, 5] = NAN
+    got = run(q, k, v, ld, s0, w, gs)
+    assert near(got["o"], clean["o"]) and near(got["dq"][:, others], clean["dq"][:, others])
+    assert near(got["dk"][:, t + 1:], clean["dk"][:, t + 1:]) and near(got["dv"][:, t + 1:], clean["dv"][:, t + 1:])
+    assert near(got["dv"][..., channels], clean["dv"][..., channels]) and near(got["dstate"][..., channels], clean["dstate"][..., channels])
+    assert bool(torch.isnan(got["dv"][:, :t + 1, :, 5]).all())
