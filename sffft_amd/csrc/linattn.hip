@@ -44,10 +44,13 @@ constexpr int MAX_JOINED = 8;
 
 // How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march, two or three
 // to a CU by their registers (half, these, double: the training step above 116.4, 114.1, 121.3; 131072 tokens of 12
-// heads of 128 channels 586, 549, 595). No more than MAX_JOINED where these still come near filling the chip and are
-// few chunks longer: a launch and the states' way through memory less. (us, bf16, 64 channels: 4 x 12 heads of 600
-// tokens 22.4 -> 17.3, 5 x 12 of 2048 39.4 -> 30.8, 2 x 12 of 2048 29.5 -> 24.4, but of 8192 45.6 -> 57; 128
-// channels: 4 x 12 of 600 40.4 -> 34.5, 8 of 1000 26.7 -> 30.7.)
+// heads of 128 channels 586, 549, 595). No more than MAX_JOINED where these are few chunks longer and as many
+// workgroups as the chip runs well: a launch and the states' way through memory less. Measured at 180 sizes of 8 to 96
+// heads and 300 to 8192 tokens, forward, time with any number of segments over time with 8: from 160 workgroups (5 for
+// every 8 CUs) on 1.0 to 1.3, of 40 to 130 0.64 to 1.14, most below 1. Above 64 channels a second workgroup on a CU
+// costs more than the launch (bf16, 2048 tokens: 36 heads, 288 workgroups 55.9 -> 66.9 us; 1200 tokens, 252 45.6 ->
+// 40.1), and segments two or more chunks longer only pay in fp32. Up to 64 channels it does not, up to three longer
+// ones either (bf16 0.94 to 1.32); fp32's third does (576 to 768 workgroups 0.85 to 1.04).
 struct Cut {
   int nseg, seg;
 };
@@ -58,7 +61,9 @@ Cut cut_of(const sffft_linattn* p, int marches) {
   const int want = (int)std::min<long long>(chunks, std::max<long long>(1, fill / heads));
   const int few = (chunks + MAX_JOINED - 1) / MAX_JOINED, joined = (chunks + few - 1) / few;
   int per = (chunks + want - 1) / want;
-  if (few > per && few - per <= (D > 64 ? 1 : 3) && joined * heads >= (D > 64 ? 240 : 192)) per = few;
+  const long long cus = 256, workgroups = joined * heads;
+  const bool fits = workgroups >= cus * 5 / 8 && (D > 64 ? workgroups <= cus : p->io || workgroups <= 2 * cus);
+  if (few > per && few - per <= (D > 64 ? 1 : 3) && fits) per = few;
   return {(chunks + per - 1) / per, per * C};
 }
 
