@@ -29,3 +29,11 @@ def dev():
     if not torch.cuda.is_available():
         pytest.fail("GPU test run without a visible GPU")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(autouse=True)
+def same_draws():
+    """What a test draws without a generator of its own is the same in every run (the GPU's default one starts anywhere)."""
+    torch = sys.modules.get("torch")
+    if torch is not None:
+        torch.manual_seed(0)
