@@ -82,14 +82,13 @@ hipError_t launch(la::Launch& L, hipStream_t st) {
                      dim3(256), 0, st, L);
   return hipGetLastError();
 }
-// Tiles of 32, 64, 96 or 128 channels of K, 64 or 128 of V. (In the next larger one instead, training, 8 x 12 heads
-// of 600 tokens, us: bf16 heads of 32 channels 51 for 45, of 96 94 for 83; fp32 95 for 68, 230 for 207.) fp32 takes
-// 128 of V up to 96 of K: the planes of more leave no room for a second workgroup on a CU (two tiles of 64 of V
-// instead: 170 us for 151 at 64 x 96 channels, 209 for 178 at 96 x 96). bf16 takes two tiles of 64 of V beside 64 of
-// K, whose outputs leave as whole rows (one of 128: 0.89 to 1.10 times as fast), and one of 128 beside more (two: 700
-// us against 570 for 131072 tokens).
+// Tiles of 32, 64, 96 or 128 channels of K, 64 or 128 of V. (In the next larger one of K instead, training, 8 x 12
+// heads of 600 tokens, us: bf16 heads of 32 channels 58 for 51, of 96 107 for 96; fp32 95 for 74, 227 for 168.) One tile
+// of 128 of V wherever it leaves two workgroups on a CU: beside fp32's 128 of K the planes do not, beside 32 of K two of
+// 64 leave three. (Two of 64 instead, us: fp32 64 x 96 channels 157 for 139, 96 x 96 199 for 169; bf16 64 x 96 104 for
+// 100, 64 x 128 of 8 x 2048 tokens 229 for 210, 128 x 128 of 131072 tokens forward 706 for 576.)
 int v_tile(int elem, int K, int V) {
-  const bool wide = elem == 4 ? K > 32 && K <= 96 : K > 64;
+  const bool wide = K > 32 && (elem == 2 || K <= 96);
   return V > 64 && wide ? 128 : 64;
 }
 template <class T, class TO, bool OUT, int UP>
@@ -97,9 +96,7 @@ hipError_t march_planes(la::Launch& L, hipStream_t st) {
   const int K = L.m[0].K;
   const bool wide = v_tile(sizeof(T), K, L.m[0].V) == 128;
   if (K <= 32) return launch<T, TO, 32, 64, OUT, UP>(L, st);
-  if constexpr (sizeof(T) == 4)
-    if (K <= 64 && wide) return launch<T, TO, 64, 128, OUT, UP>(L, st);
-  if (K <= 64) return launch<T, TO, 64, 64, OUT, UP>(L, st);
+  if (K <= 64) return wide ? launch<T, TO, 64, 128, OUT, UP>(L, st) : launch<T, TO, 64, 64, OUT, UP>(L, st);
   if (K <= 96) return wide ? launch<T, TO, 96, 128, OUT, UP>(L, st) : launch<T, TO, 96, 64, OUT, UP>(L, st);
   if constexpr (sizeof(T) == 2)
     if (wide) return launch<T, TO, 128, 128, OUT, UP>(L, st);
