@@ -57,3 +57,38 @@ def test_rotary_of_2_to_the_24_tokens(dev):
     for a in range(0, T, 1 << 20):
         z = slice(a, a + (1 << 20))
         assert torch.equal(out[:, z], torch.ops.sffft.rotary(q[:, z], q[:, z, :0], table, pos[:, z])[0]), a
+
+
+def test_attention_beyond_2_to_the_32_bytes(dev):
+    """Arrays of 4.8 GB: their last sequence gives, forward and backward, what it gives alone (in another cut: to the
+    rounding of bf16, root mean square under 2^-9 on both sides)."""
+    B, T, H, D = 48, 65536, 12, 64
+    g = torch.Generator(device=dev).manual_seed(4)
+    q, k, v, go = (torch.randn(B, T, H, D, generator=g, device=dev, dtype=torch.bfloat16) for _ in range(4))
+    ld = torch.linspace(-0.1, -0.0001, H, device=dev)
+
+    def run(z):
+        x = [t[z].requires_grad_() for t in (q, k, v)]
+        o, s = torch.ops.sffft.linear_attention(*x, ld, 0.125)
+        return (o.detach(), s.detach(), *torch.autograd.grad(o, x, go[z]))
+
+    for name, a, b in zip(("o", "state", "dq", "dk", "dv"), run(slice(0, B)), run(slice(B - 1, B))):
+        a, b = a[-1:].double(), b.double()
+        assert float((a - b).norm() / b.norm()) < (1e-5 if name == "state" else 2.0 ** -8), name
+
+
+def test_norms_beyond_2_to_the_32_bytes(dev):
+    """Rows of odd width, 4.7 GB of them: the last ones as by themselves."""
+    B, C = 1535 * 1000, 1531
+    g = torch.Generator(device=dev).manual_seed(5)
+    x, y = (torch.randn(B, C, generator=g, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    gate, w = y.flip(1), torch.rand(C, generator=g, device=dev) + 0.5
+
+    def run(z):
+        t = [u[z].requires_grad_() for u in (x, y, gate)]
+        r, h = torch.ops.sffft.block_norm(t[0], t[1], w, w, t[2], None, "silu")
+        return (r.detach(), h.detach(), *torch.autograd.grad((r, h), t, (x[z], y[z])))
+
+    for name, a, b in zip(("r", "h", "dx", "dy", "dgate"), run(slice(0, B)), run(slice(B - 1000, B))):
+        a, b = a[-1000:].double(), b.double()
+        assert float((a - b).norm() / b.norm()) < 2.0 ** -8, name
