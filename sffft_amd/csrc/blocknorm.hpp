@@ -9,10 +9,12 @@
 // stored value is rounded, and the weights' gradients would be off by that rounding.
 //
 // A row lies in the registers of one workgroup, 8 channels to a lane (16 beyond 8192 channels): every array crosses
-// memory once. Rows of up to 256 channels take 16 or 32 lanes of a wavefront, which has several of them. A workgroup
-// takes a run of rows and reads the next one before it works on this one (up to 4096 channels); sums over rows stay
-// in registers until its end, and the parts it leaves are added by a second kernel in a fixed order. Bound by memory:
-// 16384 x 4 rows of 1536 in bf16, gate for each token, 561 us forward and backward for 2.6 GB.
+// memory once. Rows of up to 256 channels take 16 or 32 lanes of a wavefront, which has several of them. Rows of
+// more than 4096 channels leave a lane 128 registers: their gradients spill up to 87 of them, beyond 8192 channels
+// up to 312 (25 M bf16 elements, gradients alone, us: C = 4096 118, 8192 178, 12288 444). A workgroup takes a run of
+// rows and reads the next one before it works on this one (up to 4096 channels); sums over rows stay in registers
+// until its end, and the parts it leaves are added by a second kernel in a fixed order. Bound by memory: 16384 x 4
+// rows of 1536 in bf16, gate for each token, 561 us forward and backward for 2.6 GB.
 //
 // Rows of an odd width start anywhere between 16-byte boundaries. A workgroup then takes rows that start at the same
 // distance from one (every 2nd, 4th or 8th) and reads them from the boundary before the row on: the vectors stay
@@ -482,8 +484,9 @@ __global__ __launch_bounds__(BLK < 64 ? 64 : BLK) void bwd_kernel(Args A) {
   }
 }
 
-// The sums of the parts (37 MB, 1024 parts of three quantities of 1531 channels: 7 us). Workgroups take 32 columns of
-// one quantity: the nparts parts of dwq and of t, which gives dwp and ds, then for each gate that rows share its
+// The sums of the parts (1024 parts of three quantities of 1531 channels: 19 MB in 7 us; rows of such widths start
+// between cache lines, and the 32 columns of a workgroup lie in two of them: 37 MB are fetched). Workgroups take 32
+// columns of one quantity: the nparts parts of dwq and of t, which gives dwp and ds, then for each gate that rows share its
 // `per` consecutive parts. There may be more quantities than the grid has rows.
 struct SumArgs {
   const float *parts, *wp, *sc;

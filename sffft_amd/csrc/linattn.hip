@@ -38,13 +38,13 @@ bool valid_input(const void* x, const long long s[3], const sffft_linattn* p, in
 Operand operand(const void* x, const long long s[3], int div) { return {x, s[0], s[1], s[2], div}; }
 
 // More segments than this are joined by a launch of its own, fewer by each workgroup that follows them. (us at 4, 8,
-// 16: training, 8 x 2048 tokens, 12 heads of 64 channels, bf16 118.5, 114.1, 114.3; 5 x 1237 tokens forward 24.3,
-// 24.5, 27.4; training, 3 x 1531 tokens, 12 heads on 4 of 96 and 64, fp32 164.3, 162.2, 188.4.)
+// 16: training, 8 x 2048 tokens, 12 heads of 64 channels, bf16 134, 130, 130; 5 x 1237 tokens forward 27.9, 26.9,
+// 29.1; training, 3 x 1531 tokens, 12 heads on 4 of 96 and 64, fp32 147, 147, 164.)
 constexpr int MAX_JOINED = 8;
 
 // How a call is cut: segments of whole chunks, as many as give the chip `fill` workgroups of the march, two or three
-// to a CU by their registers (half, these, double: the training step above 116.4, 114.1, 121.3; 131072 tokens of 12
-// heads of 128 channels 586, 549, 595). No more than MAX_JOINED where these are few chunks longer and as many
+// to a CU by their registers (half, these, double: the bf16 training step above 142, 130, 135, the fp32 one 146, 147,
+// 172; 131072 tokens of 12 heads of 128 channels 666, 576, 616). No more than MAX_JOINED where these are few chunks longer and as many
 // workgroups as the chip runs well: a launch and the states' way through memory less. Measured at 180 sizes of 8 to 96
 // heads and 300 to 8192 tokens, forward, time with any number of segments over time with 8: from 160 workgroups (5 for
 // every 8 CUs) on 1.0 to 1.3, of 40 to 130 0.64 to 1.14, most below 1. Above 64 channels a second workgroup on a CU
@@ -68,7 +68,7 @@ Cut cut_of(const sffft_linattn* p, int marches) {
 }
 
 // Marches of the gradients' smallest launch (see backward): they share one where sizes and types are equal. (Segments
-// for three marches also where each has a launch of its own: the fp32 step above 196 us instead of 162.)
+// for three marches also where each has a launch of its own: the fp32 step above 182 us instead of 147.)
 int backward_marches(const sffft_linattn* p) { return p->Dk == p->Dv && (p->H == p->Hk || !p->io) ? 3 : 1; }
 
 // Workgroups of nm marches over units of a head and a segment.
@@ -130,7 +130,7 @@ size_t state_bytes(const sffft_linattn* p, const Cut& c) {
   return c.nseg == 1 ? 0 : (size_t)p->B * p->H * c.nseg * p->Dk * p->Dv * 4;
 }
 // From this many segments on the sum of the last one is made too, for the last state: it costs one more of many sums,
-// and the march then adds to its state only what outputs of 16 bits need. (Never: 115.4, 25.1 and 164 us in the cases
+// and the march then adds to its state only what outputs of 16 bits need. (Never: 130.7, 27.5 and 146 us in the cases
 // above.)
 constexpr int MIN_ALL = 4;
 // dk and dv of heads that are shared, for each query head, before their sum

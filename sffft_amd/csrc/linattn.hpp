@@ -16,15 +16,16 @@
 //
 // Operands in 16 bits: bf16 inputs are exact. P and the entering state, operands of products that are rounded to bf16
 // in the end, are split into two bf16 parts (17 bits: 2^-9 of that rounding), one product each; in one part each they
-// made the outputs' error 2.3e-3 where their own rounding is 1.7e-3. The state is fp32 and so are the decayed c_j that
-// are added to it: they are split into three bf16 parts (8 bits each, 24 together), into two where the state only
-// serves outputs of 16 bits. fp32 inputs are split so too, and every product of two split operands is the six
-// partial products above 2^-24 (a bf16 product at 1240 TFLOP/s, an fp32 one at 154).
+// made the outputs' error 2.3e-3 where their own rounding is 1.7e-3, and training 5 to 10% faster. The state is fp32 and
+// so are the decayed c_j that are added to it: they are split into three bf16 parts (8 bits each, 24 together), into two
+// where the state only serves outputs of 16 bits (three there: the same outputs, 1 to 8% slower). fp32 inputs are split
+// so too, and every product of two split operands is the six partial products above 2^-24 (a bf16 product at 1240
+// TFLOP/s, an fp32 one at 154).
 //
-// Measured (bf16, us): 131072 tokens, 12 heads of 128: 549, sums 160 and march 368 at 4.5 TB/s, bound by memory (k
-// and v are read twice); training, 8 x 2048 tokens, 12 heads of 64: 114, sums 13 and 18, march 25 forward and 58 for
-// the gradients, bound by the chain of a chunk's products and barriers with three workgroups on a CU; one token of 96
-// x 12 heads of 128: 26, 5.9 TB/s of states.
+// Measured (bf16, us): 131072 tokens, 12 heads of 128: 577, in a trace sums 177, scan 14 and march 389 at 4.2 TB/s,
+// bound by memory (k and v are read twice); training, 8 x 2048 tokens, 12 heads of 64: 130, in a trace sums 13 and 18,
+// march 29 forward and 76 for the gradients, whose time is the chain of a chunk's products and barriers with three
+// workgroups on a CU; one token of 96 x 12 heads of 128: 26, 5.9 TB/s of states.
 #pragma once
 #include "opsio.hpp"
 
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   };
 
   // A chunk token by token, straight from memory: where a product is infinite or NaN the tiles of P that are 0 would
-  // carry it to tokens that must not see it. `from`: the chunk's first token, of which `count` count; rows: those of the
+  // carry it to tokens that must not see it. (Looking for such values takes 1 to 3% of a training step.) `from`: the chunk's first token, of which `count` count; rows: those of the
   // output. The state goes through LDS, 16 columns of a wavefront at a time, where the tiles of a, b and c are dead
   // (P's keep their zeros), so that no register is held for this.
   auto by_token = [&](int from, int count, int rows) {
@@ -713,7 +714,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
 }
 
 // The states that enter the segments, from the sums of those before them, in place. Lane: four elements. Sixteen
-// segments are read ahead. Bound by memory: 42 segments of 12 states of 128 x 128, 67 MB, in 13 us.
+// segments are read ahead. Bound by memory: 42 segments of 12 states of 128 x 128, 67 MB, in 14 us.
 struct Scan {
   float* sums;  // [bh][nseg][n]
   const float* s0;

@@ -161,8 +161,9 @@ bool apart(const Span* in, int ni, const Span* out, int no) {
 
 // WHOLE (HALVES) where every row starts and ends at a boundary of 16 (8) bytes, SHIFTED where those of all arrays
 // start at the same distance from one of 16 (a gate that rows share is read seldom and does not count). A training
-// step over 25 M elements with a gate for each token, us: bf16 C = 1531 SINGLE 897, SHIFTED 223; 2047 903, 357; 5001
-// 986, 338; fp32 1531 312, 303; 2047 343, 435; 5001 468, 415; bf16 1028 HALVES 192, SHIFTED 248.
+// step over 25 M elements with a gate for each token, us: bf16 C = 1531 SINGLE 897, SHIFTED 223; 2047 886, 380; 5001
+// 671, 354; 8185 580, 316; 9001 1462, 734; 12289 1164, 646; fp32 1531 312, 303; 2047 343, 435; 5001 476, 467; 9001 1193,
+// 937; 12289 1030, 865; bf16 1028 HALVES 192, SHIFTED 248.
 struct RowArray {
   const void* p;
   long long stride;
