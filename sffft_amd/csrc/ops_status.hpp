@@ -38,52 +38,40 @@ inline size_t extent(const long long s[3], int B, int T, int H, int D, int elem)
 
 // Whether no element of an output is written twice. Of two strided arrays [B][T][H or Hk][D] with elements of `elem`
 // bytes: neither among their own elements nor between them; of one, with hb = 0. The dimensions are taken by ascending
-// stride, each of which has to reach beyond what the smaller ones span; arrays that share their strides, such as parts
-// of a fused projection, may lie between each other's rows, and then count as one from the stride on that exceeds their
-// distance. (A few arrangements that would be in order are refused.)
+// stride, each of which has to reach beyond what the smaller ones span. Arrays may lie between each other's rows, such
+// as parts of a fused projection: the strides that they share and that exceed their distance step over both. (A few
+// arrangements that would be in order are refused.)
 inline bool distinct(const void* a, const long long sa[3], int ha, const void* b, const long long sb[3], int hb, int B, int T,
                      int D, int elem) {
   if (hb && a > b) return distinct(b, sb, hb, a, sa, ha, B, T, D, elem);
-  const int na[3] = {B, T, ha}, nb[3] = {B, T, hb};
-  const auto spans = [&](const long long s[3], const int n[3], __int128* span) {
+  // whether dimensions of n elements at strides s step over `span` elements and each other; span: of all
+  const auto steps = [](const long long s[3], const int n[3], __int128* span) {
     int order[3] = {0, 1, 2};
     std::sort(order, order + 3, [&](int i, int j) { return s[i] < s[j]; });
-    *span = D;
     for (int i : order) {
       if (n[i] > 1 && s[i] < *span) return false;
       *span += (__int128)s[i] * (n[i] - 1);
     }
     return true;
   };
-  __int128 span_a, span_b;
-  if (!spans(sa, na, &span_a)) return false;
-  if (!hb) return true;
-  const uintptr_t bytes = (uintptr_t)b - (uintptr_t)a;
-  const __int128 gap = bytes / elem;
-  if (!spans(sb, nb, &span_b)) return false;
-  if (gap >= span_a) return true;
+  const int na[3] = {B, T, ha}, nb[3] = {B, T, hb};
+  __int128 span_a = D, span_b = D;
+  if (!steps(sa, na, &span_a) || (hb && !steps(sb, nb, &span_b))) return false;
+  const uintptr_t bytes = (uintptr_t)b - (uintptr_t)a, gap = bytes / elem;
+  if (!hb || gap >= span_a) return true;
   if (bytes % elem) return false;
+  // within a row of both: what is left without the shared dimensions
+  int in_a[3], in_b[3], shared[3];
   long long s[3];
-  int order[3] = {0, 1, 2};
   for (int i = 0; i < 3; i++) {
-    if (na[i] > 1 && nb[i] > 1 && sa[i] != sb[i]) return false;
     s[i] = na[i] > 1 ? sa[i] : sb[i];
+    const bool both = (na[i] == 1 || nb[i] == 1 || sa[i] == sb[i]) && s[i] > (__int128)gap;
+    in_a[i] = both ? 1 : na[i], in_b[i] = both ? 1 : nb[i], shared[i] = both ? std::max(na[i], nb[i]) : 1;
   }
-  std::sort(order, order + 3, [&](int i, int j) { return s[i] < s[j]; });
-  bool one = false;
   span_a = span_b = D;
-  for (int i : order) {
-    const int n = std::max(na[i], nb[i]);
-    if (n == 1) continue;
-    if (!one && s[i] > gap) {
-      if (span_a > gap) return false;
-      span_a = gap + span_b, one = true;
-    }
-    if (one && s[i] < span_a) return false;
-    span_a += (__int128)s[i] * ((one ? n : na[i]) - 1);
-    span_b += (__int128)s[i] * (nb[i] - 1);
-  }
-  return one || span_a <= gap;
+  if (!steps(sa, in_a, &span_a) || !steps(sb, in_b, &span_b) || span_a > (__int128)gap) return false;
+  __int128 span = gap + span_b;
+  return steps(s, shared, &span);
 }
 
 }  // namespace ops

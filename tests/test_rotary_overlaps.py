@@ -48,6 +48,9 @@ USUAL = [  # B, T, H, Hk, D, q's strides, k's, k's place: what models have
     (1, 1, 4, 2, 8, (1, 1, 8), (7, 9, 8), 32),
     (2, 5, 4, 4, 8, (5 * 64, 64, 16), (5 * 64, 64, 16), 8),                 # heads of q and k by turns
     (2, 5, 4, 2, 8, (160, 32, 8), (80, 16, 8), 1000),                       # arrays of their own
+    (2, 5, 4, 2, 8, (5 * 64, 64, 8), (5 * 64, 64, 16), 32),                 # keys and values by turns behind the queries
+    (2, 5, 4, 2, 8, (5 * 64, 64, 8), (5 * 64, 64, 16), 40),
+    (2, 1, 4, 1, 8, (64, 3, 8), (64, 7, 3), 32),                            # one token of each
 ]
 
 
