@@ -91,7 +91,7 @@ __device__ __forceinline__ float decay_power(float l2, int n) {
   return n < 0 ? 0.f : __builtin_amdgcn_exp2f(n == 0 ? 0.f : l2 * (float)n);
 }
 // The decay over n tokens for states that pass it many times over. Rounded to fp32 it would be off by the same part of
-// itself each time, 1e-4 after 4096 chunks of a slow head; next() makes up in each factor for what the ones before it
+// itself each time, 8e-5 after 2048 chunks of a slow head; next() makes up in each factor for what the ones before it
 // left out. (A head that forgets half of its state or more in n tokens keeps no such error.)
 struct Decay {
   float hi, lo, inv;  // the decay is hi + lo
@@ -502,9 +502,10 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   };
 
   // A chunk token by token, straight from memory: where a product is infinite or NaN the tiles of P that are 0 would
-  // carry it to tokens that must not see it. (Looking for such values takes 1 to 3% of a training step.) `from`: the chunk's first token, of which `count` count; rows: those of the
-  // output. The state goes through LDS, 16 columns of a wavefront at a time, where the tiles of a, b and c are dead
-  // (P's keep their zeros), so that no register is held for this.
+  // carry it to tokens that must not see it. (Looking for such values takes 1 to 3% of a training step.) `from`: the
+  // chunk's first token, of which `count` count; rows: those of the output. The state goes through LDS, 16 columns
+  // of a wavefront at a time, where the tiles of a, b and c are dead (P's keep their zeros), so that no register is
+  // held for this.
   auto by_token = [&](int from, int count, int rows) {
     static_assert(!OUT || sizeof(tiles) - sizeof(tp) >= KT * 64 * sizeof(float), "");
     float* X = reinterpret_cast<float*>(&tiles) + (w * KT + 4 * g) * 16 + i16;
