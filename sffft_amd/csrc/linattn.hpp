@@ -508,30 +508,32 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
   // held for this.
   auto by_token = [&](int from, int count, int rows) {
     static_assert(!OUT || sizeof(tiles) - sizeof(tp) >= KT * 64 * sizeof(float), "");
-    float* X = reinterpret_cast<float*>(&tiles) + (w * KT + 4 * g) * 16 + i16;
+    float* X = reinterpret_cast<float*>(&tiles) + w * KT * 16 + i16;  // row kk of the wavefront's 16 columns at X + 16 kk
     const float decay = power(1), before = rev ? 1.f : decay, after = rev ? decay : 1.f;
 #pragma unroll
     for (int v = 0; v < VW; v++) {
 #pragma unroll
       for (int a = 0; a < KA; a++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) X[(16 * a + e) * 16] = S[a][v][e];
+        for (int e = 0; e < 4; e++) X[(16 * a + 4 * g + e) * 16] = S[a][v][e];
       const int vv = sv0 + 16 * v;
-      const T *ra = token(m.a, from) + 4 * g, *rb = token(m.b, from) + 4 * g, *rc = token(m.c, from) + vv;
+      const T *ra = token(m.a, from), *rb = token(m.b, from), *rc = token(m.c, from) + vv;
 #pragma unroll 1
       for (int s = 0; s < rows; s++) {
         const int i = rev && s < count ? count - 1 - s : s;
         const float c = s < count && vv < m.V ? m.w * ops::to_f32(rc[i * m.c.st]) : 0.f;
         float sum = 0.f;
 #pragma unroll 1
-        for (int k = s < count ? 4 * g : m.K; k < m.K; k += 16)
-#pragma unroll 1
+        for (int k = s < count ? 4 * g : m.K; k < m.K; k += 16) {
+          const T *a = ra + i * m.a.st + k, *b = rb + i * m.b.st + k;
+#pragma unroll 2
           for (int e = 0; e < 4; e++) {
-            float& x = X[(k - 4 * g + e) * 16];
-            const float y = x * before + ops::to_f32(rb[i * m.b.st + k - 4 * g + e]) * c;
-            sum += ops::to_f32(ra[i * m.a.st + k - 4 * g + e]) * y;
+            float& x = X[(k + e) * 16];
+            const float y = x * before + ops::to_f32(b[e]) * c;
+            sum += ops::to_f32(a[e]) * y;
             x = y * after;
           }
+        }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         if (g == 0 && vv < m.V) ops::put(po + (long long)i * orow + vv, m.x * sum);
@@ -539,7 +541,7 @@ __global__ __launch_bounds__(256, KT <= 64 && VT == 64 ? 3 : 2) void march_kerne
 #pragma unroll
       for (int a = 0; a < KA; a++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) S[a][v][e] = X[(16 * a + e) * 16];
+        for (int e = 0; e < 4; e++) S[a][v][e] = X[(16 * a + 4 * g + e) * 16];
     }
   };
 
